@@ -101,7 +101,7 @@ def _quantise(x):
     """x fp32 [..., d] -> codes uint8 [..., d / 2], scales fp16 [..., d / 64, 2]."""
     g = x.unflatten(-1, (-1, 64))
     lo, hi = g.amin(-1), g.amax(-1)
-    s, m = ((hi - lo) / 15).half(), lo.half()
+    s, m = ((hi - lo) / torch.full_like(hi, 15)).half(), lo.half()        # (a division: by a number, torch multiplies by its reciprocal)
     sf, mf = s.float().unsqueeze(-1), m.float().unsqueeze(-1)
     q = torch.where(sf > 0, torch.round((g - mf) / sf).clamp(0, 15), torch.zeros_like(g)).to(torch.uint8)     # [..., groups, 64]
     q = q.unflatten(-1, (8, 8)).transpose(-3, -2).flatten(-3)                                                 # words of the groups in turn
