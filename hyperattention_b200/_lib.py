@@ -56,6 +56,23 @@ class CausalParams(C.Structure):
     ]
 
 
+class PagedParams(C.Structure):
+    _fields_ = [
+        ('dtype', i32), ('bits', i32),
+        ('B', i32), ('n', i32), ('H', i32), ('Hk', i32), ('d', i32),
+        ('pages', i32), ('page_size', i32), ('columns', i32),
+        ('rot', i32), ('rope_rows', i32), ('rope_dtype', i32), ('rows', i32), ('scale', f32), ('reserved', i32),
+        ('q', vp), ('k', vp), ('v', vp),
+        ('q_sb', i64), ('q_sn', i64), ('q_sh', i64), ('k_sb', i64), ('k_sn', i64), ('k_sh', i64),
+        ('v_sb', i64), ('v_sn', i64), ('v_sh', i64),
+        ('k_pages', vp), ('v_pages', vp), ('page_sp', i64), ('page_sh', i64), ('page_st', i64),
+        ('k_scales', vp), ('v_scales', vp), ('scale_sp', i64), ('scale_sh', i64), ('scale_st', i64),
+        ('table', vp), ('table_sb', i64), ('lengths', vp), ('counts', vp), ('rope', vp),
+        ('q_out', vp), ('k_out', vp), ('v_out', vp), ('o', vp), ('lse', vp),
+        ('workspace', vp), ('workspace_bytes', i64), ('status', vp), ('status_host', vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/hyperattn_b200.h declares
 SIGNATURES = {
     'ha_version': (C.c_char_p, []),
@@ -88,6 +105,10 @@ SIGNATURES = {
     'ha_uniform_sample': (C.c_int, [i32, i32, i32, C.c_uint64, vp, vp]),
     'ha_flash_bwd_scratch_bytes': (i64, [C.POINTER(AttnParams), vp]),
     'ha_flash_bwd': (C.c_int, [C.POINTER(AttnParams), vp, vp, vp, vp, i64, vp]),
+    'ha_paged_append': (C.c_int, [C.POINTER(PagedParams), vp]),
+    'ha_paged_attn_workspace_bytes': (i64, [C.POINTER(PagedParams)]),
+    'ha_paged_attn': (C.c_int, [C.POINTER(PagedParams), vp]),
+    'ha_paged_gather': (C.c_int, [C.POINTER(PagedParams), vp]),
     'ha_wait_probe': (C.c_int, [vp, vp, i32, vp]),
     'ha_causal_saved_bytes': (i64, [C.POINTER(CausalParams)]),
     'ha_causal_scratch_bytes': (i64, [C.POINTER(CausalParams), i32]),

@@ -289,6 +289,61 @@ int ha_uniform_sample(int32_t rows, int32_t n, int32_t sample_size, uint64_t bas
 int64_t ha_flash_bwd_scratch_bytes(const ha_attn_params* p, const void* dq);
 int ha_flash_bwd(const ha_attn_params* p, void* dq, void* dk, void* dv, void* scratch, int64_t scratch_bytes, void* stream);
 
+/* --------------------------------------------------------------------------------------------------------------
+ * Generation with a paged key/value cache.  No counterpart in the reference, whose attention covers prompts only.
+ *
+ * The cache is a pool of pages; a page holds page_size token rows of every K/V head.
+ *   bits = 16: k_pages, v_pages [pages][Hk][page_size][d] in `dtype`, element strides page_sp, page_sh, page_st (equal for both; rows
+ *              contiguous; rows on 16-byte boundaries).
+ *   bits = 4:  codes, uint8 [pages][Hk][page_size][d / 2], strides in bytes, and k_scales, v_scales fp16 [pages][Hk][page_size][d / 64][2] with
+ *              strides scale_sp, scale_sh, scale_st in elements (rows contiguous, on 8-byte boundaries for d = 128, 4-byte ones for d = 64).
+ *              A group of 64 elements x: s = fp16((max - min) / 15), m = fp16(min), code = clamp(rint((x - m) / s), 0, 15), 0 where s = 0, all
+ *              in 32 bits; it stands for code * s + m.  A group whose s or m fp16 cannot hold (a NaN, an infinity, a span over 15 * 65504) has
+ *              s = 0, m = NaN.  Eight neighbours share a 32-bit word, nibble i the i-th; with d = 128 the words of the two groups alternate.
+ * table: int32 [B] rows of `columns` page numbers, table_sb elements apart: position t of sequence b lies in page table[b][t / page_size],
+ * row t % page_size.  Entries behind a sequence's last page are not read.  A position beyond the table, beyond the rotation's rows,
+ * or in a page that does not exist sets the status words to HA_DEV_BAD_INDEX; its row is neither written nor read.
+ * dtype HA_BF16 or HA_FP16; d 64 or 128; H a multiple of Hk. */
+typedef struct ha_paged_params {
+  int32_t dtype, bits;
+  int32_t B, n, H, Hk, d;                 /* n: new tokens of each sequence */
+  int32_t pages, page_size, columns;
+  int32_t rot, rope_rows, rope_dtype;     /* rotation: elements of a row, positions, HA_FP32 or `dtype` */
+  int32_t rows;                           /* ha_paged_gather */
+  float scale;
+  int32_t reserved;
+  const void *q, *k, *v;                  /* [B][n][H or Hk][d], element strides, rows contiguous */
+  int64_t q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh;
+  void *k_pages, *v_pages;
+  int64_t page_sp, page_sh, page_st;
+  void *k_scales, *v_scales;
+  int64_t scale_sp, scale_sh, scale_st;
+  const int32_t *table;
+  int64_t table_sb;
+  const int32_t *lengths, *counts;        /* int32 [B]; counts may be NULL: n each */
+  const void *rope;                       /* [rope_rows][rot / 2][2] cosine, sine; NULL: no rotation */
+  void *q_out, *k_out, *v_out;
+  void *o;                                /* [B][n][H][d], contiguous */
+  float *lse;                             /* [B][H][n] */
+  void *workspace;
+  int64_t workspace_bytes;
+  int32_t *status, *status_host;
+} ha_paged_params;
+
+/* Row i < counts[b] of k and v goes to position lengths[b] + i of sequence b, the first `rot` elements of k rotated there: pairs (2j, 2j+1),
+ * (x0 c - x1 s, x1 c + x0 s), every product and sum rounded to 32 bits, the result once more to `dtype` (4 bits: the codes are taken from the 32-bit values).
+ * q (may be NULL) is rotated alike into q_out [B][n][H][d]; k_out (may be NULL) [B][n][Hk][d] gets the rotated keys too; rows i >= counts[b] of both
+ * are zero.  Two rows of one call must not name the same slot. */
+int ha_paged_append(const ha_paged_params* p, void* stream);
+
+/* Query row i < counts[b] attends to positions 0 .. lengths[b] - counts[b] + i: lengths counts the rows of this call, too.  o and natural-log lse as
+ * the other attention entry points give them; a row without keys, and rows i >= counts[b], have o = 0, lse = -infinity.  q on 16-byte rows. */
+int64_t ha_paged_attn_workspace_bytes(const ha_paged_params* p);
+int ha_paged_attn(const ha_paged_params* p, void* stream);
+
+/* Positions 0 .. rows - 1 of every sequence as dense [B][Hk][rows][d] tensors k_out, v_out in `dtype`; zero from lengths[b] on. */
+int ha_paged_gather(const ha_paged_params* p, void* stream);
+
 /* Diagnostic for the timeout path.  One warp polls an mbarrier that nothing ever arrives at, `polls` times (1..2^18),
  * gives up and reports HA_DEV_TIMEOUT through status / status_host exactly as the attention kernels do when one of their
  * bounded waits runs out.  No copy and no tensor-core operation is in flight; the kernel returns normally and the
