@@ -69,7 +69,7 @@ class PagedParams(C.Structure):
         ('k_scales', vp), ('v_scales', vp), ('scale_sp', i64), ('scale_sh', i64), ('scale_st', i64),
         ('table', vp), ('table_sb', i64), ('lengths', vp), ('counts', vp), ('rope', vp),
         ('q_out', vp), ('k_out', vp), ('v_out', vp), ('o', vp), ('lse', vp),
-        ('workspace', vp), ('workspace_bytes', i64), ('status', vp), ('status_host', vp),
+        ('workspace', vp), ('workspace_bytes', i64), ('status', vp), ('status_host', vp), ('maps', vp),
     ]
 
 
@@ -105,6 +105,7 @@ SIGNATURES = {
     'ha_uniform_sample': (C.c_int, [i32, i32, i32, C.c_uint64, vp, vp]),
     'ha_flash_bwd_scratch_bytes': (i64, [C.POINTER(AttnParams), vp]),
     'ha_flash_bwd': (C.c_int, [C.POINTER(AttnParams), vp, vp, vp, vp, i64, vp]),
+    'ha_paged_maps': (C.c_int, [C.POINTER(PagedParams), vp]),
     'ha_paged_append': (C.c_int, [C.POINTER(PagedParams), vp]),
     'ha_paged_attn_workspace_bytes': (i64, [C.POINTER(PagedParams)]),
     'ha_paged_attn': (C.c_int, [C.POINTER(PagedParams), vp]),

@@ -58,9 +58,10 @@ inline void launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t s
 __device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // First statement of every thread of a chained kernel: waits until the previous kernel is complete and its memory operations are visible.  Nothing is
 // read or written before it, so that what lies further back in the stream is complete, too.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_begin() {
   chain_release();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  chain_wait();
 }
 
 inline int dtype_size(int dtype) { return dtype == HA_FP32 ? 4 : 2; }

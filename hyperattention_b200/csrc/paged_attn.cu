@@ -11,18 +11,24 @@
 // finished there; of one that crosses to the next, each CTA writes its part (unnormalised sums, reference, denominator) to the workspace,
 // and paged_combine_kernel adds them up in the order of the keys.  A CTA's own parts of an item: at most the first and the last of its list.
 //
-// A CTA of four warps; each warp takes a quarter of a tile's keys with its own running maximum and sums, which are joined at the item's end.  Tiles
-// come by cp.async in a ring of NS stages, across items; queries come with the first tile of an item.
+// A CTA: four warps that compute, each a quarter of a tile's keys with its own running maximum and sums, which are joined at the item's end; and one that
+// fetches tiles into a ring of NS stages, across items: 16-bit rows by tensor copies (128-byte swizzle; boxes of as many rows as both a page and a
+// tile are made of, so that any page size will do), 4-bit rows by plain bulk copies, queries and scales by cp.async.
+#include <string.h>
+
+#include <numeric>
 #include <type_traits>
 
 #include "paged.cuh"
+#include "tensor_map.cuh"
 
 namespace ha {
 
 namespace {
 
 constexpr int ITEM_ROWS = 16;
-constexpr int MAX_LINES = 416;        // (sequence, token) pairs of one launch: their tiles are summed up in shared memory
+constexpr int MAX_LINES = 256;        // (sequence, token) pairs of one launch: their tiles are summed up in shared memory
+constexpr int THREADS = 160;
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 
 struct AttnArgs {
@@ -33,8 +39,10 @@ struct AttnArgs {
   float* lse;
   int32_t n, H, Hk, group, blocks;    // blocks: items of a (token, K/V head): group / 16, rounded up
   int32_t line0, lines;               // (sequence, token) pairs of this launch
+  int32_t run_log2;                   // rows that are fetched together: 2^run_log2, the largest power of two that pages and tiles are made of
   FastDiv by_n, by_blocks;
-  float scale_log2;
+  float scale_log2;                   // magnitude of the softmax scale, times log2 e
+  uint32_t flip;                      // sign bits of a pair of queries, where the scale is negative
   float* part;                        // [CTAs][2][ITEM_ROWS][D], then ...
   float2* part_stat;                  // [CTAs][2][ITEM_ROWS]: reference (log2), denominator
   int4* head;                         // [CTAs]: last item's first and end tile, its line, its number
@@ -47,15 +55,16 @@ struct Stage {
   static constexpr int TK = 4 * KW;
   static constexpr int ROW = BITS == 16 ? 2 * D : D / 2;     // bytes of a row
   static constexpr int G = D / PAGED_GROUP;
-  static constexpr int SC = BITS == 16 ? 0 : 4 * G;
-  static constexpr int V = TK * ROW, KS = 2 * TK * ROW, VS = KS + TK * SC, Q = VS + TK * SC;
+  static constexpr int SC = BITS == 16 ? 4 : 4 * G;          // bytes of a row's scales (16 bits: none)
+  static constexpr int V = TK * ROW, KS = 2 * TK * ROW, VS = KS + (BITS == 16 ? 0 : TK * SC), Q = VS + (BITS == 16 ? 0 : TK * SC);
   static constexpr int BYTES = Q + ITEM_ROWS * 2 * D;
-  static constexpr int NS = BITS == 16 ? (D == 128 ? 3 : 6) : (D == 128 ? 3 : 5);
-  static constexpr int CTAS = BITS == 16 ? 2 : 3;
-  static constexpr int RING = 2 * TK * (BITS == 16 ? 8 : 16);
+  static constexpr int CTAS = BITS == 16 ? (D == 128 ? 2 : 3) : 2;
+  static constexpr int NS = BITS == 16 ? (D == 128 ? 3 : 4) : (D == 128 ? 4 : 8);
   static constexpr int ROUNDS = BITS == 16 ? 1 : 2;          // in which the warps' sums are joined: column ranges that fit a stage
-  static constexpr int SMEM = NS * BYTES + RING + 4 * ITEM_ROWS * 8 + (2 * MAX_LINES + 1) * 4 + 32;
+  static constexpr int BARS = 2 * NS + 1;
+  static constexpr int SMEM = NS * BYTES + 4 * ITEM_ROWS * 8 + BARS * 8 + (2 * MAX_LINES + 8) * 4 + 16;
   static_assert(4 * ITEM_ROWS * D / ROUNDS * 4 <= Q, "the warps' sums fit a stage");
+  static_assert(BYTES % (BITS == 16 ? 1024 : 128) == 0, "stages begin on the swizzle's boundary");
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
@@ -63,41 +72,36 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 template <int N>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, uint32_t src_bytes) {      // 4 or 8 bytes
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(src_bytes) : "memory");
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ uint2 lds64(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
+__device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
+// contiguous bytes (16-byte aligned, a multiple of 16) to shared memory, counted on `bar`
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
+// an arrival on `bar` once this thread's cp.async so far are done
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ uint64_t dup_f2(float v) { return pack_f2(v, v); }
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -106,12 +110,15 @@ __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-// 16-byte chunk of a row in shared memory: the eight rows that one ldmatrix phase (or one quarter of a 128-bit load) touches lie in different banks
+// 16-bit rows in shared memory: 128-byte slabs of 64 elements, 16-byte chunk c of row r at chunk c ^ (r & 7): the eight rows that one ldmatrix
+// phase (or one quarter of a 128-bit load) touches lie in different banks.  Queries: whole rows, chunks turned alike.
+template <int TK>
+__device__ __forceinline__ uint32_t slab_at(int row, int chunk) { return (chunk >> 3) * (TK * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }
-// 4-bit rows of 64 bytes: K lies in the order in which the score columns name keys (column 2c + e is key c + 4e of its eight), V in key order, its 16-byte
-// chunks turned so that the four keys c .. of one 64-bit load fill all banks
+// 4-bit rows lie in key order.  Column 2c + e of a score fragment is key c + 4e of its eight: the four keys that one load of V takes then are
+// neighbours, two to a bank instead of four.  Scales lie in column order: a lane's two keys side by side.
 __device__ __forceinline__ int column_of(int key) { return (key & ~7) | ((key & 3) << 1) | ((key >> 2) & 1); }
-template <int D> __device__ __forceinline__ int v4_chunk(int key, int chunk) { return D == 128 ? chunk ^ (((key >> 1) & 1) << 1) : chunk; }
+__device__ __forceinline__ int key_of(int column) { return (column >> 1) | ((column & 1) << 2); }
 
 // A place in the list of tiles.
 struct Walk {
@@ -133,32 +140,38 @@ template <typename T, int D, int BITS>
 struct Worker {
   using S = Stage<D, BITS>;
   static constexpr int NT = S::KW / 8;        // score fragments (eight keys each) of a warp's part of a tile
-  static constexpr float BIAS = 15.f;         // (fp16 weights) of the reference: weights up to 2^15, normal down to 2^-29 of the largest
+  // (fp16 weights) weights reach up to 2^15 and stay normal down to 2^-29 of the largest
+  static constexpr float BIAS = BITS == 4 || std::is_same<T, __half>::value ? 15.f : 0.f;
 
-  // of rows lane / 4 and lane / 4 + 8
-  float ref[2], sum[2];
+  // of rows lane / 4 and lane / 4 + 8.  Weights are exp2(score - shift); 16 bits: ref is the largest product q . k so far, shift = ref * scale - BIAS;
+  // 4 bits: ref is the largest score so far, shift = ref + v_exp - BIAS, so that weight * step stays within fp16, too
+  float ref[2], shift[2];
+  uint64_t sum[2];                            // (even columns, odd columns)
   float acc[D / 8][4];
   uint32_t qf[D / 16][4];
   // 4-bit rows
   float q_unit[2], q_sum[S::G][2];            // score of a code sum; sum of the row's elements of a group, times the softmax scale
-  float weight[S::G][4];                      // sums of the rounded weights (every column alike)
-  float offset[S::G][2];                      // sum of weights times what a row's middle code stands for
+  float weight[S::G][4];                      // sums of the rounded weights of even columns, less those of odd ones (every column alike)
+  uint64_t offset[S::G][2];                   // sums of weights times what a row's middle code stands for
   float v_exp;                                // power of two that no V step so far exceeds
 
-  __device__ __forceinline__ void begin(uint32_t stage, float scale_log2) {
+  __device__ __forceinline__ void begin(const uint8_t* stage, const AttnArgs& a) {
     const int lane = threadIdx.x & 31;
     ref[0] = ref[1] = -INFINITY;
-    sum[0] = sum[1] = 0.f;
+    shift[0] = shift[1] = 0.f;
+    sum[0] = sum[1] = 0;
 #pragma unroll
     for (int j = 0; j < D / 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    const uint32_t q = stage + S::Q;
+    const uint8_t* q = stage + S::Q;
     if constexpr (BITS == 16) {
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const int row = lane & 15;
-        ldmatrix4(qf[ks], q + row * 2 * D + chunk_at(row, 2 * ks + (lane >> 4)) * 16);
+        ldmatrix4(qf[ks], smem_u32(q) + row * 2 * D + chunk_at(row, 2 * ks + (lane >> 4)) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[ks][e] ^= a.flip;
       }
     } else {
       // Queries as fp16 operands: every row times the power of two that brings its largest element to 2^13 .. 2^14.  Lane c of a row's four
@@ -175,7 +188,7 @@ struct Worker {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint4 w = lds128(q + row * 2 * D + chunk_at(row, 8 * g + 2 * c + u) * 16);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+            const uint32_t ws[4] = {w.x ^ a.flip, w.y ^ a.flip, w.z ^ a.flip, w.w ^ a.flip};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float2 f = unpack2<T>(ws[j]);
@@ -185,9 +198,9 @@ struct Worker {
               top = max_nan(top, max_nan(fabsf(f.x), fabsf(f.y)));
             }
           }
-          q_sum[g][half] = quad_sum(s) * scale_log2;
+          q_sum[g][half] = quad_sum(s) * a.scale_log2;
           weight[g][2 * half] = weight[g][2 * half + 1] = 0.f;
-          offset[g][half] = 0.f;
+          offset[g][half] = 0;
         }
         top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -195,7 +208,7 @@ struct Worker {
         const int e = max((int)(__float_as_uint(top) >> 23) & 255, 27);
         const float up = __uint_as_float((uint32_t)(127 + 13 + 127 - e) << 23), down = __uint_as_float((uint32_t)(e - 13) << 23);
         // codes are the subnormal fp16 numbers code * 2^-24 (or * 2^-20, against a sixteenth of the query's element)
-        q_unit[half] = down * 16777216.f * scale_log2;
+        q_unit[half] = down * 16777216.f * a.scale_log2;
 #pragma unroll
         for (int g = 0; g < S::G; ++g)
 #pragma unroll
@@ -210,55 +223,57 @@ struct Worker {
     }
   }
 
-  // new reference of the rows whose maximum grew; the sums so far follow
-  __device__ __forceinline__ void raise(const float (&top)[2], float v_top) {
+  // New reference of the rows whose maximum grew (and of all, where a V step did); the sums so far follow.
+  __device__ __forceinline__ void raise(const float (&top)[2], float v_top, float scale_log2) {
     float by[2];
-    float exp_new = 0.f, exp_old = 0.f;
     if constexpr (BITS == 4) {
-      exp_old = v_exp;
 #pragma unroll
       for (int s = 1; s < 32; s *= 2) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, s));
       v_exp = fmaxf(v_exp, (float)((int)(__float_as_uint(v_top) >> 23) - 126));
-      exp_new = v_exp;
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float now = fmaxf(ref[r], quad_max(top[r]));
-      by[r] = now == -INFINITY ? 1.f : fast_exp2((ref[r] - now) + (exp_old - exp_new));
-      ref[r] = now;
-      sum[r] *= by[r];
+      const bool empty = ref[r] == -INFINITY;
+      ref[r] = fmaxf(ref[r], quad_max(top[r]));
+      const float now = ref[r] == -INFINITY ? 0.f : BITS == 4 ? ref[r] + (v_exp - BIAS) : fmaf(ref[r], scale_log2, -BIAS);
+      by[r] = empty ? 0.f : fast_exp2(shift[r] - now);
+      // (sums of a row without a score so far are zeros, or NaN)
+      shift[r] = now;
+      sum[r] = fmul2(sum[r], dup_f2(by[r]));
     }
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      acc[j][0] *= by[0];
-      acc[j][1] *= by[0];
-      acc[j][2] *= by[1];
-      acc[j][3] *= by[1];
-    }
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] *= by[e >> 1];
     if constexpr (BITS == 4) {
 #pragma unroll
       for (int g = 0; g < S::G; ++g) {
-        weight[g][0] *= by[0];
-        weight[g][2] *= by[1];
-        offset[g][0] *= by[0];
-        offset[g][1] *= by[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) weight[g][e] *= by[e >> 1];
+        offset[g][0] = fmul2(offset[g][0], dup_f2(by[0]));
+        offset[g][1] = fmul2(offset[g][1], dup_f2(by[1]));
       }
     }
   }
-  // what is taken off a score's exponent: weights are exp2(x - shift)
-  __device__ __forceinline__ float shift(int r) const {
-    if (ref[r] == -INFINITY) return 0.f;
-    if constexpr (BITS == 4) return ref[r] + v_exp - BIAS;
-    else return std::is_same<T, __half>::value ? ref[r] - BIAS : ref[r];
+
+  // Rows of V (4 bits: their scales) behind the last key hold anything: zeros instead.
+  __device__ __forceinline__ void clear_tail(uint8_t* stage, int left) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    left = max(left, 0);
+    if constexpr (BITS == 16) {
+      for (int e = left * (D / 8) + lane; e < S::KW * (D / 8); e += 32) *reinterpret_cast<uint4*>(stage + S::V + slab_at<S::TK>(warp * S::KW + e / (D / 8), e % (D / 8))) = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int e = left * S::G + lane; e < S::KW * S::G; e += 32) *reinterpret_cast<uint32_t*>(stage + S::VS + column_of(warp * S::KW + e / S::G) * S::SC + e % S::G * 4) = 0;
+    }
+    __syncwarp();
   }
 
-  // One tile: this warp's keys are left .. left + KW - 1 (of the row's `left` that are still to come, counted from this warp's first).
-  __device__ __forceinline__ void tile(uint32_t stage, int left, float scale_log2) {
+  // One tile: this warp's keys, of which the first `left` exist.
+  __device__ __forceinline__ void tile(const uint8_t* stage, int left, float scale_log2) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
-    float x[NT][4];
     if constexpr (BITS == 16) {
-      const int row = warp * 16 + (lane & 7) + ((lane >> 4) << 3);
-      const uint32_t k = stage + row * S::ROW;
+      float x[NT][4];
+      const int row = warp * S::KW + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -266,84 +281,127 @@ struct Worker {
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         uint32_t b[4];
-        ldmatrix4(b, k + chunk_at(row, 2 * ks + ((lane >> 3) & 1)) * 16);
+        ldmatrix4(b, smem_u32(stage) + slab_at<S::TK>(row, 2 * ks + ((lane >> 3) & 1)));
         mma16816<T>(x[0], qf[ks], b[0], b[1]);
         mma16816<T>(x[1], qf[ks], b[2], b[3]);
       }
+      if (left < S::KW) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t * 8 + 2 * c + (e & 1) >= left) x[t][e] = -INFINITY;
+      }
+      const float top[2] = {fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]))};
+      if (__any_sync(0xffffffffu, top[0] > ref[0] || top[1] > ref[1])) raise(top, 0.f, scale_log2);
+      // Weights as the sum of two numbers of T: the second holds what the first rounds off, so that the output's own rounding is the one that
+      // counts.  The products are far from the bound (a second one costs nothing that the loads do not hide).
+      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[t][e] *= scale_log2;
-          if (left < S::KW && t * 8 + 2 * c + (e & 1) >= left) x[t][e] = -INFINITY;
+        for (int r = 0; r < 2; ++r) {
+          float p0, p1;
+          unpack_f2(ffma2(pack_f2(x[t][2 * r], x[t][2 * r + 1]), dup_f2(scale_log2), dup_f2(-shift[r])), p0, p1);
+          p0 = fast_exp2(p0);
+          p1 = fast_exp2(p1);
+          sum[r] = fadd2(sum[r], pack_f2(p0, p1));
+          const uint32_t w = pack2<T>(p0, p1);
+          const float2 f = unpack2<T>(w);
+          hi[2 * t + r] = w;
+          lo[2 * t + r] = pack2<T>(p0 - f.x, p1 - f.y);
         }
+      const int vrow = warp * S::KW + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t b[4];
+        ldmatrix4t(b, smem_u32(stage) + S::V + slab_at<S::TK>(vrow, 2 * j + (lane >> 4)));
+        mma16816<T>(acc[2 * j], hi, b[0], b[1]);
+        mma16816<T>(acc[2 * j + 1], hi, b[2], b[3]);
+        mma16816<T>(acc[2 * j], lo, b[0], b[1]);
+        mma16816<T>(acc[2 * j + 1], lo, b[2], b[3]);
+      }
     } else {
+      uint64_t x[NT][2];                       // scores less shift, of two keys, of a row
+      const uint64_t below[2] = {dup_f2(-shift[0]), dup_f2(-shift[1])};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int at = warp * 32 + t * 8;
-        uint32_t w[4];
-        if constexpr (D == 128) {
-          const uint4 v = lds128(stage + (at + lane / 4) * S::ROW + c * 16);
-          w[0] = v.x, w[1] = v.z, w[2] = v.y, w[3] = v.w;                // words of the first group, of the second
-        } else {
-          const uint2 v = lds64(stage + (at + lane / 4) * S::ROW + c * 8);
-          w[0] = v.x, w[1] = v.y;
-        }
-        float d[S::G][4];
+      for (int t2 = 0; t2 < NT; t2 += 2) {
+        uint32_t w[2][2 * S::G], sc[2][2][S::G];                         // words of the groups in turn; of this lane's two keys: step, value of code 0
+        float d[2][S::G][4];
 #pragma unroll
-        for (int g = 0; g < S::G; ++g) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[g][e] = 0.f;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t a = w[2 * g + u], b = a >> 8;
-            mma16816<__half>(d[g], qf[(g * 2 + u) * 2], a & 0x000f000fu, a & 0x00f000f0u);
-            mma16816<__half>(d[g], qf[(g * 2 + u) * 2 + 1], b & 0x000f000fu, b & 0x00f000f0u);
+        for (int v = 0; v < 2; ++v) {
+          const int at = warp * S::KW + (t2 + v) * 8;
+          if constexpr (D == 128) {
+            const uint4 f = lds128(stage + (at + key_of(lane / 4)) * S::ROW + c * 16), f2 = lds128(stage + S::KS + (at + 2 * c) * S::SC);
+            w[v][0] = f.x, w[v][1] = f.y, w[v][2] = f.z, w[v][3] = f.w;
+            sc[v][0][0] = f2.x, sc[v][0][1] = f2.y, sc[v][1][0] = f2.z, sc[v][1][1] = f2.w;
+          } else {
+            const uint2 f = lds64(stage + (at + key_of(lane / 4)) * S::ROW + c * 8), f2 = lds64(stage + S::KS + (at + 2 * c) * S::SC);
+            w[v][0] = f.x, w[v][1] = f.y;
+            sc[v][0][0] = f2.x, sc[v][1][0] = f2.y;
           }
-        }
-        uint32_t sc[2][S::G];                                            // of this lane's two keys
-        if constexpr (D == 128) {
-          const uint4 v = lds128(stage + S::KS + (at + 2 * c) * S::SC);
-          sc[0][0] = v.x, sc[0][1] = v.y, sc[1][0] = v.z, sc[1][1] = v.w;
-        } else {
-          const uint2 v = lds64(stage + S::KS + (at + 2 * c) * S::SC);
-          sc[0][0] = v.x, sc[1][0] = v.y;
-        }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float y[2] = {0.f, 0.f}, z[2] = {0.f, 0.f};
+          for (int g = 0; g < S::G; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[v][g][e] = 0.f;
+        }
+        // (the products of one sum a few others apart)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int x8 = 0; x8 < 2; ++x8)
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+              for (int g = 0; g < S::G; ++g) {
+                const uint32_t a = w[v][u * S::G + g] >> (8 * x8);
+                mma16816<__half>(d[v][g], qf[(g * 2 + u) * 2 + x8], a & 0x000f000fu, a & 0x00f000f0u);
+              }
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          uint64_t y[2], z[2] = {below[0], below[1]};
 #pragma unroll
           for (int g = 0; g < S::G; ++g) {
-            const float2 f = unpack2<__half>(sc[e][g]);                  // step, value of code 0
+            const float2 f0 = unpack2<__half>(sc[v][0][g]), f1 = unpack2<__half>(sc[v][1][g]);
+            const uint64_t step = pack_f2(f0.x, f1.x), zero = pack_f2(f0.y, f1.y);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              y[r] = g == 0 ? f.x * d[g][2 * r + e] : fmaf(f.x, d[g][2 * r + e], y[r]);
-              z[r] = g == 0 ? f.y * q_sum[g][r] : fmaf(f.y, q_sum[g][r], z[r]);
+              const uint64_t dd = pack_f2(d[v][g][2 * r], d[v][g][2 * r + 1]);
+              y[r] = g == 0 ? fmul2(step, dd) : ffma2(step, dd, y[r]);
+              z[r] = ffma2(zero, dup_f2(q_sum[g][r]), z[r]);
             }
           }
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            x[t][2 * r + e] = fmaf(y[r], q_unit[r], z[r]);
-            if (left < S::KW && t * 8 + c + 4 * e >= left) x[t][2 * r + e] = -INFINITY;
-          }
+          for (int r = 0; r < 2; ++r) x[t2 + v][r] = ffma2(y[r], dup_f2(q_unit[r]), z[r]);
         }
       }
-    }
-
-    float top[2] = {fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])};
+      if (left < S::KW) {
 #pragma unroll
-    for (int t = 1; t < NT; ++t) {
-      top[0] = fmax3(top[0], x[t][0], x[t][1]);
-      top[1] = fmax3(top[1], x[t][2], x[t][3]);
-    }
-    uint32_t vsc[NT][2][S::G];
-    float v_top = 0.f;
-    bool grew = top[0] > ref[0] || top[1] > ref[1];
-    if constexpr (BITS == 4) {
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float x0, x1;
+            unpack_f2(x[t][r], x0, x1);
+            x[t][r] = pack_f2(t * 8 + c < left ? x0 : -INFINITY, t * 8 + c + 4 < left ? x1 : -INFINITY);
+          }
+      }
+      float top[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float x0, x1;
+        unpack_f2(x[0][r], x0, x1);
+        top[r] = fmaxf(x0, x1);
+#pragma unroll
+        for (int t = 1; t < NT; ++t) {
+          unpack_f2(x[t][r], x0, x1);
+          top[r] = fmax3(top[r], x0, x1);
+        }
+      }
+      uint32_t vsc[NT][2][S::G];
       __half2 most = __half2half2(__ushort_as_half(0));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int at = warp * 32 + t * 8 + 2 * c;
+        const int at = warp * S::KW + t * 8 + 2 * c;
         if constexpr (D == 128) {
           const uint4 v = lds128(stage + S::VS + at * S::SC);
           vsc[t][0][0] = v.x, vsc[t][0][1] = v.y, vsc[t][1][0] = v.z, vsc[t][1][1] = v.w;
@@ -356,48 +414,34 @@ struct Worker {
 #pragma unroll
           for (int g = 0; g < S::G; ++g) most = __hmax2(most, *reinterpret_cast<const __half2*>(&vsc[t][e][g]));
       }
-      v_top = __low2float(most);
-      grew = grew || v_top >= exp2f_int(v_exp);
-    }
-    if (__any_sync(0xffffffffu, grew)) raise(top, v_top);
-    const float sh[2] = {shift(0), shift(1)};
+      const float v_top = __low2float(most);
+      // (score > ref, as scores less shift; a row without scores has ref -inf and shift 0)
+      const bool grew = top[0] + shift[0] > ref[0] || top[1] + shift[1] > ref[1] || v_top >= __uint_as_float((uint32_t)((int)v_exp + 127) << 23);
+      if (__any_sync(0xffffffffu, grew)) {
+        const float old[2] = {shift[0], shift[1]};
+        top[0] += old[0];
+        top[1] += old[1];
+        raise(top, v_top, scale_log2);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[t][e] = fast_exp2(x[t][e] - sh[e >> 1]);
-        sum[e >> 1] += x[t][e];
+          for (int r = 0; r < 2; ++r) x[t][r] = fadd2(x[t][r], dup_f2(old[r] - shift[r]));
       }
-
-    if constexpr (BITS == 16) {
-      // Weights as the sum of two numbers of T: the second holds what the first rounds off, so that the output's own rounding is the one that
-      // counts.  The products are far from the bound (a second one costs nothing that the loads do not hide).
-      uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t w = pack2<T>(x[t][2 * r], x[t][2 * r + 1]);
-          const float2 f = unpack2<T>(w);
-          hi[2 * t + r] = w;
-          lo[2 * t + r] = pack2<T>(x[t][2 * r] - f.x, x[t][2 * r + 1] - f.y);
+          float p0, p1;
+          unpack_f2(x[t][r], p0, p1);
+          x[t][r] = pack_f2(fast_exp2(p0), fast_exp2(p1));
+          sum[r] = fadd2(sum[r], x[t][r]);
         }
-      const int row = warp * 16 + (lane & 15);
-      const uint32_t v = stage + S::V + row * S::ROW;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        uint32_t b[4];
-        ldmatrix4t(b, v + chunk_at(row, 2 * j + (lane >> 4)) * 16);
-        mma16816<T>(acc[2 * j], hi, b[0], b[1]);
-        mma16816<T>(acc[2 * j + 1], hi, b[2], b[3]);
-        mma16816<T>(acc[2 * j], lo, b[0], b[1]);
-        mma16816<T>(acc[2 * j + 1], lo, b[2], b[3]);
-      }
-    } else {
 #pragma unroll
       for (int u = 0; u < NT / 2; ++u) {
-        // weight times step, rounded to fp16; what the middle code stands for is added in 32 bits, and the rounded weights are summed up by
-        // the same products, so that a rounding meets (code - 7.5) and not the code
+        // Weight times step, rounded to fp16.  What the middle code stands for is added in 32 bits, and the rounded weights are summed up by the
+        // same products, so that a rounding meets (code - 7.5) and not the code.  Keys of odd columns enter as 15 - code with the weight's sign
+        // turned: the sums stay near the middle, where tensor cores, which cut sums off instead of rounding them, lose nothing that counts
+        // (262144 keys, fp16 output: error 1.3e-3 with plain codes).
         uint32_t p[S::G][4];
 #pragma unroll
         for (int g = 0; g < S::G; ++g)
@@ -405,19 +449,21 @@ struct Worker {
           for (int h = 0; h < 2; ++h) {
             const int t = 2 * u + h;
             const float2 f0 = unpack2<__half>(vsc[t][0][g]), f1 = unpack2<__half>(vsc[t][1][g]);
-            const float m0 = fmaf(7.5f, f0.x, f0.y), m1 = fmaf(7.5f, f1.x, f1.y);
+            const uint64_t step = pack_f2(f0.x, -f1.x), mid = ffma2(step, pack_f2(7.5f, -7.5f), pack_f2(f0.y, f1.y));
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              p[g][2 * h + r] = pack2<__half>(x[t][2 * r] * f0.x, x[t][2 * r + 1] * f1.x);
-              offset[g][r] = fmaf(x[t][2 * r], m0, fmaf(x[t][2 * r + 1], m1, offset[g][r]));
+              float a, b;
+              unpack_f2(fmul2(x[t][r], step), a, b);
+              p[g][2 * h + r] = pack2<__half>(a, b);
+              offset[g][r] = ffma2(x[t][r], mid, offset[g][r]);
             }
           }
         uint32_t w[4][S::G];                                             // keys c, c + 4 of the first eight, of the second
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const int key = warp * 32 + u * 16 + (y >> 1) * 8 + c + 4 * (y & 1);
+          const int key = warp * S::KW + u * 16 + (y >> 1) * 8 + c + 4 * (y & 1);
           if constexpr (D == 128) {
-            const uint2 v = lds64(stage + S::V + key * S::ROW + v4_chunk<D>(key, lane >> 3) * 16 + ((lane >> 2) & 1) * 8);
+            const uint2 v = lds64(stage + S::V + key * S::ROW + (lane >> 2) * 8);
             w[y][0] = v.x, w[y][1] = v.y;
           } else {
             w[y][0] = lds32(stage + S::V + key * S::ROW + (lane >> 2) * 4);
@@ -430,17 +476,32 @@ struct Worker {
           for (int h = 0; h < 2; ++h) {                                  // elements 0 - 3, 4 - 7 of the words
             const uint32_t sel = h ? 0x7632u : 0x5410u;
             const uint32_t a = __byte_perm(w[0][g], w[1][g], sel), b = __byte_perm(w[2][g], w[3][g], sel), a8 = a >> 8, b8 = b >> 8;
+            constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u, X0 = 0x000f0000u, X1 = 0x00f00000u;
             float(*o)[4] = acc + g * 8 + h * 4;
-            mma16816<__half>(o[0], p[g], a & 0x000f000fu, b & 0x000f000fu);
-            mma16816<__half>(o[1], p[g], a & 0x00f000f0u, b & 0x00f000f0u);
-            mma16816<__half>(o[2], p[g], a8 & 0x000f000fu, b8 & 0x000f000fu);
-            mma16816<__half>(o[3], p[g], a8 & 0x00f000f0u, b8 & 0x00f000f0u);
+            mma16816<__half>(o[0], p[g], (a & M0) ^ X0, (b & M0) ^ X0);
+            mma16816<__half>(o[1], p[g], (a & M1) ^ X1, (b & M1) ^ X1);
+            mma16816<__half>(o[2], p[g], (a8 & M0) ^ X0, (b8 & M0) ^ X0);
+            mma16816<__half>(o[3], p[g], (a8 & M1) ^ X1, (b8 & M1) ^ X1);
           }
         }
       }
     }
   }
-  static __device__ __forceinline__ float exp2f_int(float e) { return __uint_as_float((uint32_t)((int)e + 127) << 23); }
+
+  // The lane's partial sums become the row's.
+  __device__ __forceinline__ float finish(int r) {
+    float a, b;
+    unpack_f2(sum[r], a, b);
+    if constexpr (BITS == 4) {
+#pragma unroll
+      for (int g = 0; g < S::G; ++g) {
+        float u, v;
+        unpack_f2(offset[g][r], u, v);
+        offset[g][r] = pack_f2(quad_sum(u + v), 0.f);
+      }
+    }
+    return quad_sum(a + b);
+  }
 
   // This warp's sums of columns [round * D / ROUNDS ..) in the stage, rows of D / ROUNDS floats; columns of 8 turned by the row.
   __device__ __forceinline__ void put(float* to, int round) {
@@ -458,7 +519,9 @@ struct Worker {
 #pragma unroll
         for (int g = 0; g < S::G; ++g) {
           if (S::G == S::ROUNDS && g != round) continue;
-          const float mid = offset[g][half] - 7.5f * weight[g][2 * half];
+          float mid, none;
+          unpack_f2(offset[g][half], mid, none);
+          mid = fmaf(-7.5f, weight[g][2 * half], mid);
 #pragma unroll
           for (int j = 0; j < 8; j += 2)
 #pragma unroll
@@ -474,23 +537,128 @@ struct Worker {
   }
 };
 
-template <typename T, int D, int BITS>
-__global__ void __launch_bounds__(128, Stage<D, BITS>::CTAS) paged_attn_kernel(const AttnArgs a) {
+// The warp that fetches: tiles begin .. end - 1 into the ring.  full[s]: every lane arrives once its copies are there; empty[s]: the four warps that compute.
+template <int D, int BITS>
+__device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, const int* first, const int* keys, Walk at,
+                                            int begin, int end, int items, uint32_t base, uint32_t bars, int* abort_flag) {
   using S = Stage<D, BITS>;
   constexpr int NS = S::NS, TK = S::TK;
-  extern __shared__ __align__(128) uint8_t smem[];
-  int64_t* ring = reinterpret_cast<int64_t*>(smem + NS * S::BYTES);          // [2][TK] offsets of rows, -1: none; 4 bits: [2][TK] of their scales, too
-  float2* stat = reinterpret_cast<float2*>(smem + NS * S::BYTES + S::RING);  // [4][ITEM_ROWS]
+  const int lane = threadIdx.x & 31, run = 1 << a.run_log2;
+  // page and slot of the run `r` of a tile; page -1: no key there, or no page
+  auto look_up = [&](const Walk& w, int r, int& slot) {
+    slot = 0;
+    const int key = w.tile * TK + (r << a.run_log2);
+    if (w.line >= a.lines || (r << a.run_log2) >= TK || key >= keys[w.line]) return -1;
+    return paged_slot(a.c, a.by_n(a.line0 + w.line), key, slot);
+  };
+  int slot, page = look_up(at, lane, slot);
+  int s = 0;
+  uint32_t round = 0;
+  for (int it = begin; it < end; ++it) {
+    const uint32_t full = bars + 8 * s, empty = bars + 8 * (NS + s), dst = base + s * S::BYTES;
+    if (round > 0 && !mbar_wait_or_abort(empty, (round - 1) & 1, abort_flag)) break;
+    Walk next = at;
+    next.step(first, a.lines, items);
+    if (it + 1 == end) next.line = a.lines;
+    int next_slot;
+    const int next_page = look_up(next, lane, next_slot);              // (under way while this tile's copies are started)
+    const int b = a.by_n(a.line0 + at.line), i = a.line0 + at.line - b * a.n;
+    const int h = a.by_blocks(at.item), left = keys[at.line] - at.tile * TK;
+    for (int r0 = 0; (r0 << a.run_log2) < min(TK, left); r0 += 32) {
+      if (r0 > 0) page = look_up(at, r0 + lane, slot);                 // (runs of less than TK / 32 rows)
+      const int row = (r0 + lane) << a.run_log2;
+      if (page >= 0) {
+        if constexpr (BITS == 16) {
+          mbar_add_tx(full, 2 * S::ROW << a.run_log2);
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) {
+            tma_tile(dst + x * TK * 128 + row * 128, km, 64 * x, slot, h, page, full);
+            tma_tile(dst + S::V + x * TK * 128 + row * 128, vm, 64 * x, slot, h, page, full);
+          }
+        } else {
+          const int64_t off = page * a.c.sp + h * a.c.sh + slot * a.c.st;
+          const int rows = min(run, left - row);
+          mbar_add_tx(full, 2 * S::ROW * rows);
+          if (a.c.st == S::ROW) {
+            bulk_copy(dst + row * S::ROW, a.c.k + off, rows * S::ROW, full);
+            bulk_copy(dst + S::V + row * S::ROW, a.c.v + off, rows * S::ROW, full);
+          } else {
+            for (int y = 0; y < rows; ++y) {
+              bulk_copy(dst + (row + y) * S::ROW, a.c.k + off + y * a.c.st, S::ROW, full);
+              bulk_copy(dst + S::V + (row + y) * S::ROW, a.c.v + off + y * a.c.st, S::ROW, full);
+            }
+          }
+        }
+      }
+      if constexpr (BITS == 4) {
+        // scales of the rows of these 32 runs, a lane a row
+        const int rows = min(32 << a.run_log2, TK);
+        for (int y = lane; y < rows; y += 32) {
+          const int q = y >> a.run_log2;
+          const int pg = __shfl_sync(0xffffffffu, page, q), sl = __shfl_sync(0xffffffffu, slot, q) + (y & (run - 1));
+          const int to = column_of((r0 << a.run_log2) + y);
+          const int64_t off = pg >= 0 ? pg * a.c.ssp + h * a.c.ssh + sl * a.c.sst : 0;
+          const uint32_t bytes = pg >= 0 ? S::SC : 0;
+          cp_async_small<S::SC>(dst + S::KS + to * S::SC, a.c.ks + off, bytes);
+          cp_async_small<S::SC>(dst + S::VS + to * S::SC, a.c.vs + off, bytes);
+        }
+      }
+    }
+    if (it == begin || at.tile == 0) {
+      const int block = at.item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
+      const uint8_t* q = a.q + b * a.q_sb + i * a.q_sn + (int64_t)(h * a.group + block * ITEM_ROWS) * a.q_sh;
+      constexpr int C = 2 * D / 16;
+#pragma unroll
+      for (int e = lane; e < ITEM_ROWS * C; e += 32) {
+        const int r = e / C, chunk = e % C;
+        cp_async16(dst + S::Q + r * 2 * D + chunk_at(r, chunk) * 16, q + (r < rows ? r : 0) * a.q_sh + chunk * 16, r < rows ? 16 : 0);
+      }
+    }
+    cp_async_arrive(full);
+    at = next;
+    page = next_page;
+    slot = next_slot;
+    if (++s == NS) s = 0, ++round;
+  }
+  // nothing leaves while copies into its memory are under way
+  cp_async_wait<0>();
+  if (*reinterpret_cast<volatile int*>(abort_flag)) {
+    // (the last NS tiles that were started: stages s .. NS - 1 of the round before, 0 .. s - 1 of this one)
+    for (int y = 0; y < NS; ++y) {
+      const uint32_t r = y < s ? round : round - 1;
+      if (y < s || round > 0) mbar_wait(bars + 8 * y, r & 1);
+    }
+  }
+}
+
+template <typename T, int D, int BITS>
+__global__ void __launch_bounds__(THREADS, (Stage<D, BITS>::CTAS))
+    paged_attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm) {
+  using S = Stage<D, BITS>;
+  constexpr int NS = S::NS, TK = S::TK;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float2* stat = reinterpret_cast<float2*>(smem + NS * S::BYTES);            // [4][ITEM_ROWS]
   int* first = reinterpret_cast<int*>(stat + 4 * ITEM_ROWS);                 // [lines + 1] tiles before a line (of one item)
-  int* keys = first + MAX_LINES + 1;                                         // [lines]
-  int* warp_sum = keys + MAX_LINES;                                          // [4]
+  int* keys = first + MAX_LINES + 4;                                         // [lines]
+  const uint32_t base = smem_u32(smem), bars = smem_u32(keys + MAX_LINES);   // full[NS], empty[NS], join
+  int* warp_sum = keys + MAX_LINES + 2 * S::BARS;                            // [4], abort flag in the last of ...
+  int* abort_flag = first + MAX_LINES + 3;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int items = a.Hk * a.blocks;
-  chain_begin();
+  if (tid == 0) {
+    for (int y = 0; y < NS; ++y) {
+      mbar_init(bars + 8 * y, 32);
+      mbar_init(bars + 8 * (NS + y), 4);
+    }
+    mbar_init(bars + 8 * 2 * NS, 4);
+    mbar_fence_init();
+    *abort_flag = 0;
+  }
+  chain_wait();
 
-  // keys and tiles of every line: four consecutive lines a thread
+  // keys and tiles of every line: consecutive lines a thread
   {
-    constexpr int PER = (MAX_LINES + 127) / 128;
+    constexpr int PER = (MAX_LINES + 1 + 127) / 128;
     int before = 0, mine[PER];
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
@@ -512,17 +680,17 @@ __global__ void __launch_bounds__(128, Stage<D, BITS>::CTAS) paged_attn_kernel(c
     }
     int incl = before;
 #pragma unroll
-    for (int s = 1; s < 32; s *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, s);
-      if (lane >= s) incl += v;
+    for (int y = 1; y < 32; y *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, y);
+      if (lane >= y) incl += v;
     }
-    if (lane == 31) warp_sum[warp] = incl;
+    if (lane == 31 && warp < 4) warp_sum[warp] = incl;
     __syncthreads();
-    int base = incl - before;
-    for (int w = 0; w < warp; ++w) base += warp_sum[w];
+    int ahead = incl - before;
+    for (int w = 0; w < min(warp, 4); ++w) ahead += warp_sum[w];
 #pragma unroll
     for (int u = 0; u < PER; ++u)
-      if (tid * PER + u <= a.lines) first[tid * PER + u] = base + mine[u];
+      if (tid * PER + u <= a.lines) first[tid * PER + u] = ahead + mine[u];
     __syncthreads();
   }
   const int total = first[a.lines] * items;
@@ -537,12 +705,12 @@ __global__ void __launch_bounds__(128, Stage<D, BITS>::CTAS) paged_attn_kernel(c
     if (keys[line] > 0) continue;
     const int b = a.by_n(a.line0 + line), i = a.line0 + line - b * a.n;
     uint4* o = reinterpret_cast<uint4*>((T*)a.o + (int64_t)(a.line0 + line) * a.H * D);
-    for (int e = tid; e < a.H * D / 8; e += 128) o[e] = make_uint4(0, 0, 0, 0);
-    for (int h = tid; h < a.H; h += 128) a.lse[((int64_t)b * a.H + h) * a.n + i] = -INFINITY;
+    for (int e = tid; e < a.H * D / 8; e += THREADS) o[e] = make_uint4(0, 0, 0, 0);
+    for (int h = tid; h < a.H; h += THREADS) a.lse[((int64_t)b * a.H + h) * a.n + i] = -INFINITY;
   }
   if (begin >= end) return;
 
-  Walk at;                                     // tile that is computed
+  Walk at;
   {
     int lo = 0, hi = a.lines;                  // the last line whose tiles begin at or before `begin`
     while (hi - lo > 1) {
@@ -551,119 +719,45 @@ __global__ void __launch_bounds__(128, Stage<D, BITS>::CTAS) paged_attn_kernel(c
       else hi = mid;
     }
     at.line = lo;
-    at.settle(first, a.lines);                 // (lines without tiles share their first tile with the next one: the search may stop at such)
+    at.settle(first, a.lines);
     const int off = begin - first[at.line] * items;
     at.item = off / at.tiles;
     at.tile = off - at.item * at.tiles;
   }
-  Walk name = at, fetch = at;                  // tile whose rows are looked up next; tile that is fetched next
-  int named = begin, fetched = begin;
-  const uint32_t base = smem_u32(smem);
-
-  // offset of the row that this thread looks up (every thread up to TK) of tile `name`
-  auto look_up = [&](int64_t& off, int64_t& off_s) {
-    off = off_s = -1;
-    if (named < end && tid < TK) {
-      const int key = name.tile * TK + tid;
-      if (key < keys[name.line]) {
-        const int b = a.by_n(a.line0 + name.line), h = a.by_blocks(name.item);
-        int row;
-        const int page = paged_slot(a.c, b, key, row);
-        if (page >= 0) {
-          off = page * a.c.sp + h * a.c.sh + row * a.c.st;
-          if (BITS == 4) off_s = page * a.c.ssp + h * a.c.ssh + row * a.c.sst;
-        }
-      }
-    }
-  };
-  auto keep = [&](int64_t off, int64_t off_s) {
-    if (tid < TK) {
-      ring[(named & 1) * TK + tid] = off;
-      if (BITS == 4) ring[2 * TK + (named & 1) * TK + tid] = off_s;
-    }
-    if (named < end) name.step(first, a.lines, items);
-    ++named;
-  };
-  auto issue = [&]() {
-    if (fetched < end) {
-      const uint32_t dst = base + ((fetched - begin) % NS) * S::BYTES;
-      const int64_t* offs = ring + (fetched & 1) * TK;
-      if constexpr (BITS == 16) {
-        constexpr int C = S::ROW / 16, PASS = 128 / C;
-        const int chunk = tid % C;
-#pragma unroll
-        for (int r = tid / C; r < TK; r += PASS) {
-          const int64_t off = offs[r];
-          const uint32_t bytes = off >= 0 ? 16 : 0, to = dst + r * S::ROW + chunk_at(r, chunk) * 16;
-          const int64_t from = (off >= 0 ? off : 0) + chunk * 16;
-          cp_async16(to, a.c.k + from, bytes);
-          cp_async16(to + S::V, a.c.v + from, bytes);
-        }
-      } else {
-        constexpr int C = S::ROW / 16, PASS = 128 / C;
-        const int chunk = tid % C;
-#pragma unroll
-        for (int r = tid / C; r < TK; r += PASS) {
-          const int64_t off = offs[r];
-          const uint32_t bytes = off >= 0 ? 16 : 0;
-          const int64_t from = (off >= 0 ? off : 0) + chunk * 16;
-          cp_async16(dst + column_of(r) * S::ROW + chunk * 16, a.c.k + from, bytes);
-          cp_async16(dst + S::V + r * S::ROW + v4_chunk<D>(r, chunk) * 16, a.c.v + from, bytes);
-        }
-        const int64_t off = offs[2 * TK + tid];
-        const uint32_t bytes = off >= 0 ? S::SC : 0;
-        const int64_t from = off >= 0 ? off : 0;
-        cp_async_small<S::SC == 0 ? 4 : S::SC>(dst + S::KS + column_of(tid) * S::SC, a.c.ks + from, bytes);
-        cp_async_small<S::SC == 0 ? 4 : S::SC>(dst + S::VS + column_of(tid) * S::SC, a.c.vs + from, bytes);
-      }
-      if (fetched == begin || fetch.tile == 0) {
-        const int b = a.by_n(a.line0 + fetch.line), i = a.line0 + fetch.line - b * a.n;
-        const int h = a.by_blocks(fetch.item), block = fetch.item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
-        const uint8_t* q = a.q + b * a.q_sb + i * a.q_sn + (int64_t)(h * a.group + block * ITEM_ROWS) * a.q_sh;
-        constexpr int C = 2 * D / 16;
-#pragma unroll
-        for (int e = tid; e < ITEM_ROWS * C; e += 128) {
-          const int r = e / C, chunk = e % C;
-          cp_async16(dst + S::Q + r * 2 * D + chunk_at(r, chunk) * 16, q + (r < rows ? r : 0) * a.q_sh + chunk * 16, r < rows ? 16 : 0);
-        }
-      }
-      fetch.step(first, a.lines, items);
-    }
-    cp_async_commit();
-    ++fetched;
-  };
-
-  int64_t off, off_s;
-#pragma unroll 1
-  for (int s = 0; s < NS - 1; ++s) {
-    look_up(off, off_s);
-    keep(off, off_s);
-    __syncthreads();
-    issue();
+  if (warp == 4) {
+    fetch_tiles<D, BITS>(a, &km, &vm, first, keys, at, begin, end, items, base, bars, abort_flag);
+    return;
   }
-  look_up(off, off_s);
-  keep(off, off_s);
 
   Worker<T, D, BITS> w;
+  const uint32_t join_bar = bars + 8 * 2 * NS;
+  uint32_t joined = 0;
+  // all four warps are here, and what they wrote to shared memory is visible
+  auto join = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(join_bar);
+    return mbar_wait_or_abort(join_bar, joined++ & 1, abort_flag);
+  };
+  int s = 0;
+  uint32_t round = 0;
+  bool ok = true;
 #pragma unroll 1
-  for (int it = begin; it < end; ++it) {
-    cp_async_wait<NS - 2>();
-    __syncthreads();                           // tile `it` is there, its predecessor's stage free, the rows of tile it + NS - 1 named
-    issue();
-    look_up(off, off_s);                       // (its load is under way during the tile)
-    const uint32_t stage = base + ((it - begin) % NS) * S::BYTES;
-    if (it == begin || at.tile == 0) w.begin(stage, a.scale_log2);
-    w.tile(stage, keys[at.line] - at.tile * TK - warp * S::KW, a.scale_log2);
-    if (at.tile == at.tiles - 1 || it == end - 1) {
+  for (int it = begin; it < end && ok; ++it) {
+    uint8_t* stage = smem + s * S::BYTES;
+    ok = mbar_wait_or_abort(bars + 8 * s, round & 1, abort_flag);
+    if (!ok) break;
+    if (it == begin || at.tile == 0) w.begin(stage, a);
+    const int left = keys[at.line] - at.tile * TK - warp * S::KW;
+    if (left < S::KW) w.clear_tail(stage, left);
+    w.tile(stage, left, a.scale_log2);
+    const bool ends = at.tile == at.tiles - 1 || it == end - 1;
+    if (ends) {
       // The item ends, or this CTA's part of it: the warps' sums are joined.
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float l = quad_sum(w.sum[r]);
-        if (BITS == 4)
-#pragma unroll
-          for (int g = 0; g < S::G; ++g) w.offset[g][r] = quad_sum(w.offset[g][r]);
+        const float l = w.finish(r);
         // a warp without keys has no part; one whose scores are all NaN has
-        if ((lane & 3) == 0) stat[warp * ITEM_ROWS + lane / 4 + 8 * r] = make_float2(w.ref[r] == -INFINITY && l == 0.f ? -INFINITY : w.shift(r), l);
+        if ((lane & 3) == 0) stat[warp * ITEM_ROWS + lane / 4 + 8 * r] = make_float2(w.ref[r] == -INFINITY && l == 0.f ? -INFINITY : w.shift[r], l);
       }
       const int b = a.by_n(a.line0 + at.line), i = a.line0 + at.line - b * a.n;
       const int h = a.by_blocks(at.item), block = at.item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
@@ -671,13 +765,14 @@ __global__ void __launch_bounds__(128, Stage<D, BITS>::CTAS) paged_attn_kernel(c
       const bool whole = item_begin >= begin && item_end <= end;
       const int row = tid >> 3;
       constexpr int W = D / S::ROUNDS;
-      float* sums = reinterpret_cast<float*>(smem + ((it - begin) % NS) * S::BYTES);
+      float* sums = reinterpret_cast<float*>(stage);
       float part[4], m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int round = 0; round < S::ROUNDS; ++round) {
-        __syncthreads();                       // the stage has been read (the round before, too); the statistics are there
-        w.put(sums + warp * ITEM_ROWS * W, round);
-        if (round == 0) {
+      for (int y = 0; y < S::ROUNDS && ok; ++y) {
+        ok = join();                           // the stage has been read (the round before, too); the statistics are there
+        if (!ok) break;
+        w.put(sums + warp * ITEM_ROWS * W, y);
+        if (y == 0) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) m = fmaxf(m, stat[x * ITEM_ROWS + row].x);
 #pragma unroll
@@ -687,7 +782,8 @@ __global__ void __launch_bounds__(128, Stage<D, BITS>::CTAS) paged_attn_kernel(c
             if (!(part[x] < 0.f)) l = fmaf(part[x], st.y, l);
           }
         }
-        __syncthreads();
+        ok = join();
+        if (!ok) break;
         const float inv = whole ? 1.f / l : 1.f;
         const int64_t out = ((int64_t)(a.line0 + at.line) * a.H + h * a.group + block * ITEM_ROWS + row) * D;
         const int slot = 2 * blockIdx.x + (item_begin <= begin ? 0 : 1);
@@ -697,32 +793,37 @@ __global__ void __launch_bounds__(128, Stage<D, BITS>::CTAS) paged_attn_kernel(c
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const float4 y = *reinterpret_cast<const float4*>(sums + (x * ITEM_ROWS + row) * W + (col ^ ((row & 3) << 3)));
+            const float4 f = *reinterpret_cast<const float4*>(sums + (x * ITEM_ROWS + row) * W + (col ^ ((row & 3) << 3)));
             if (!(part[x] < 0.f)) {
-              v.x = fmaf(part[x], y.x, v.x);
-              v.y = fmaf(part[x], y.y, v.y);
-              v.z = fmaf(part[x], y.z, v.z);
-              v.w = fmaf(part[x], y.w, v.w);
+              v.x = fmaf(part[x], f.x, v.x);
+              v.y = fmaf(part[x], f.y, v.y);
+              v.z = fmaf(part[x], f.z, v.z);
+              v.w = fmaf(part[x], f.w, v.w);
             }
           }
           if (row < rows) {
             if (whole)
-              *reinterpret_cast<uint2*>((T*)a.o + out + round * W + col) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+              *reinterpret_cast<uint2*>((T*)a.o + out + y * W + col) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
             else
-              *reinterpret_cast<float4*>(a.part + ((int64_t)slot * ITEM_ROWS + row) * D + round * W + col) = v;
+              *reinterpret_cast<float4*>(a.part + ((int64_t)slot * ITEM_ROWS + row) * D + y * W + col) = v;
           }
         }
-        if (round == 0 && row < rows && (tid & 7) == 0) {
+        if (y == 0 && row < rows && (tid & 7) == 0) {
           if (whole) a.lse[((int64_t)b * a.H + h * a.group + block * ITEM_ROWS + row) * a.n + i] = (m + log2f(l)) * LN2;
           else a.part_stat[slot * ITEM_ROWS + row] = make_float2(m, l);
         }
       }
       if (it == end - 1 && tid == 0) a.head[blockIdx.x] = make_int4(item_begin, item_end, a.line0 + at.line, at.item);
     }
-    keep(off, off_s);
+    // the stage is free (what was written to it by stores before what copies write to it next)
+    if (ends || left < S::KW) fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars + 8 * (NS + s));
     at.step(first, a.lines, items);
+    if (++s == NS) s = 0, ++round;
   }
-  cp_async_wait<0>();
+  if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
+  chain_release();
 }
 
 // Joins the parts of the items that cross from one CTA's list to the next.  Block (c, row): the item that begins in CTA c's list and ends behind it.
@@ -730,7 +831,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const AttnArgs a) {
   __shared__ float red[4][D];
   __shared__ float red_m[4], red_l[4];
-  chain_begin();
+  chain_wait();
   const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int total = a.meta[0], per = a.meta[1];
   if ((int64_t)(c + 1) * per >= total) return;
@@ -783,12 +884,16 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const AttnArgs a) {
 }
 
 int attn_tile(const ha_paged_params& p) { return p.bits == 16 ? 64 : 128; }
+int attn_resident(const ha_paged_params& p) {
+  if (p.bits == 16) return p.d == 128 ? Stage<128, 16>::CTAS : Stage<64, 16>::CTAS;
+  return p.d == 128 ? Stage<128, 4>::CTAS : Stage<64, 4>::CTAS;
+}
 
 // CTAs of a launch over `lines` lines: as many as are resident at once, and no more than there can be tiles.
 int attn_ctas(const ha_paged_params& p, int lines) {
   const int tk = attn_tile(p), items = p.Hk * ((p.H / p.Hk + ITEM_ROWS - 1) / ITEM_ROWS);
   const int64_t most = ((int64_t)p.columns * p.page_size + tk - 1) / tk * items * lines;
-  const int resident = sm_count() * (p.bits == 16 ? 2 : 3);
+  const int resident = sm_count() * attn_resident(p);
   return (int)(most < 1 ? 1 : most < resident ? most : resident);
 }
 
@@ -801,18 +906,33 @@ int64_t attn_lines(const ha_paged_params& p) {
   return lines;
 }
 
+// Tensor maps of K and V pages: boxes of as many rows as both a page and a tile are made of.
+bool attn_maps(const ha_paged_params& p, CUtensorMap* maps) {
+  if (p.pages == 0) return true;
+  const int run = std::gcd(p.page_size, 64);
+  const int64_t row = p.page_size == 1 ? p.d : p.page_st;
+  return encode_tile_map(&maps[0], p.dtype, p.k_pages, p.d, p.page_size, p.Hk, p.pages, row, p.page_sh, p.page_sp, run) &&
+         encode_tile_map(&maps[1], p.dtype, p.v_pages, p.d, p.page_size, p.Hk, p.pages, row, p.page_sh, p.page_sp, run);
+}
+
 int64_t attn_workspace(const ha_paged_params& p, int ctas) { return 256 + (int64_t)ctas * (16 + 2 * ITEM_ROWS * (p.d * 4 + 8)); }
 
 template <typename T, int D, int BITS>
 int launch_attn(AttnArgs a, const ha_paged_params& p, cudaStream_t st) {
   using S = Stage<D, BITS>;
+  while ((1 << a.run_log2) < std::gcd(p.page_size, S::TK)) ++a.run_log2;
+  CUtensorMap maps[2] = {};
+  if (BITS == 16) {
+    if (p.maps) memcpy(maps, p.maps, sizeof(maps));
+    else if (!attn_maps(p, maps)) return HA_ERR_INVALID;
+  }
   HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D, BITS>), S::SMEM, "ha_paged_attn");
   const int64_t all = (int64_t)p.B * p.n, most = attn_lines(p);
   for (int64_t line0 = 0; line0 < all; line0 += most) {
     a.line0 = (int)line0;
     a.lines = (int)(all - line0 < most ? all - line0 : most);
     const int ctas = attn_ctas(p, a.lines);
-    launch_chained(paged_attn_kernel<T, D, BITS>, ctas, 128, S::SMEM, st, a);
+    launch_chained(paged_attn_kernel<T, D, BITS>, ctas, THREADS, S::SMEM, st, a, maps[0], maps[1]);
     HA_LAUNCHED("ha_paged_attn");
     if (ctas > 1) {
       launch_chained(paged_combine_kernel<T, D>, dim3(ctas - 1, a.group < ITEM_ROWS ? a.group : ITEM_ROWS), 128, 0, st, a);
@@ -825,7 +945,7 @@ int launch_attn(AttnArgs a, const ha_paged_params& p, cudaStream_t st) {
 int attn_check(const ha_paged_params& p) {
   const int rc = paged_check(p);
   if (rc != HA_OK) return rc;
-  if (p.H < 1) return HA_ERR_INVALID;
+  if (p.H < 1 || p.scale == 0.f) return HA_ERR_INVALID;
   if ((int64_t)p.B * p.n > 0x7fffffffLL - 65536 || (int64_t)p.H * p.d > 1 << 24) return HA_ERR_TOO_LARGE;
   if (p.B > 0 && p.n > 0 && attn_lines(p) < 1) return HA_ERR_TOO_LARGE;
   return HA_OK;
@@ -837,6 +957,19 @@ int attn_check(const ha_paged_params& p) {
 using namespace ha;
 
 extern "C" {
+
+int ha_paged_maps(const ha_paged_params* pp, void* maps) {
+  if (!pp || !maps) return HA_ERR_INVALID;
+  const ha_paged_params& p = *pp;
+  ha_paged_params q = p;
+  q.B = 0;
+  const int rc = paged_check(q);
+  if (rc != HA_OK) return rc;
+  CUtensorMap m[2] = {};
+  if (p.bits == 16 && !attn_maps(p, m)) return HA_ERR_INVALID;
+  memcpy(maps, m, sizeof(m));
+  return HA_OK;
+}
 
 int64_t ha_paged_attn_workspace_bytes(const ha_paged_params* pp) {
   if (!pp) return HA_ERR_INVALID;
@@ -866,7 +999,8 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   a.o = p.o; a.lse = p.lse;
   a.n = p.n; a.H = p.H; a.Hk = p.Hk; a.group = p.H / p.Hk; a.blocks = (a.group + ITEM_ROWS - 1) / ITEM_ROWS;
   a.by_n = FastDiv((uint32_t)p.n); a.by_blocks = FastDiv((uint32_t)a.blocks);
-  a.scale_log2 = p.scale * LOG2E;
+  a.scale_log2 = fabsf(p.scale) * LOG2E;
+  a.flip = p.scale < 0.f ? 0x80008000u : 0u;
   uint8_t* ws = (uint8_t*)p.workspace;
   a.meta = (int32_t*)ws;
   a.head = (int4*)(ws + 256);

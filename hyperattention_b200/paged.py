@@ -37,7 +37,7 @@ class PagedCache:
     the handle checks them once and keeps them."""
 
     def __init__(self, k, v, k_scales=None, v_scales=None, dtype=None):
-        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self._tensors = (k, v) if k_scales is None and v_scales is None else (k, v, k_scales, v_scales)
         self.bits = 16 if k_scales is None else 4
         assert (k_scales is None) == (v_scales is None), 'a 4-bit cache has scales of both K and V'
         assert k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device, 'K and V pages must be alike'
@@ -71,7 +71,17 @@ class PagedCache:
         p.page_sp, p.page_sh, p.page_st = k.stride()[:3]
         if self.bits == 4:
             p.scale_sp, p.scale_sh, p.scale_st = k_scales.stride()[:3]
-        self._key = bytes(p)             # the parameters of a call that the cache decides, pointers apart
+        for name, t in zip(('k_pages', 'v_pages', 'k_scales', 'v_scales'), self._tensors):
+            setattr(p, name, t.data_ptr())
+        self._raw = bytes(p)             # the parameters of a call that the cache decides
+        self._at = [t.data_ptr() for t in self._tensors]
+        self._maps = None                # what the attention kernel keeps about 16-bit pages
+        self._plans = {}                 # parameters of calls by their tensors' shapes and strides (bounded); no pointers but the cache's own
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scales = property(lambda self: self._tensors[2] if self.bits == 4 else None)
+    v_scales = property(lambda self: self._tensors[3] if self.bits == 4 else None)
 
     @classmethod
     def allocate(cls, pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, bits=16, device='cuda'):
@@ -94,34 +104,42 @@ class PagedCache:
             out.append((q * scales[..., :1].float() + scales[..., 1:].float()).flatten(-2))
         return tuple(out)
 
-    def _params(self):
-        p = L.PagedParams.from_buffer_copy(self._key)
-        p.k_pages, p.v_pages = self.k.data_ptr(), self.v.data_ptr()
-        if self.bits == 4:
-            p.k_scales, p.v_scales = self.k_scales.data_ptr(), self.v_scales.data_ptr()
-        return p
+    def _check_place(self):
+        assert [t.data_ptr() for t in self._tensors] == self._at, 'the pages have moved: make a new PagedCache'
+
+    def _plan(self, key, make):
+        """Parameters of a call whose tensors have the shapes, strides and types of `key`: checked and filled in once."""
+        plan = self._plans.get(key)
+        if plan is None:
+            p = L.PagedParams.from_buffer_copy(self._raw)
+            rest = make(p)
+            if len(self._plans) >= 256:
+                self._plans.clear()
+            plan = self._plans[key] = (bytes(p), rest)
+        return plan
+
+
+def _form(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 def _places(p, cache, table, lengths, counts, B):
-    """Fills in the table and the lengths of a call, checked."""
-    dev = cache.device
+    """Checks the table and the lengths of a call, and fills in their sizes."""
     ops._cuda(cache.k)
+    dev = cache.device
     assert table.dim() == 2 and table.shape[0] == B and table.dtype == torch.int32 and (table.stride(1) == 1 or table.shape[1] <= 1), \
         'table must be int32 [batch, columns], rows contiguous'
     assert lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.is_contiguous(), 'lengths must be contiguous int32 [batch]'
     assert table.device == dev and lengths.device == dev, 'all tensors must be on one device'
-    p.columns, p.table_sb, p.table, p.lengths = table.shape[1], table.stride(0), table.data_ptr(), lengths.data_ptr()
     if counts is not None:
         assert counts.shape == (B,) and counts.dtype == torch.int32 and counts.is_contiguous() and counts.device == dev, \
             'counts must be contiguous int32 [batch]'
-        p.counts = counts.data_ptr()
-    ops._set_status(p, dev)
+    p.B, p.columns, p.table_sb = B, table.shape[1], table.stride(0)
 
 
 def _rows(cache, t, B, n, heads, what):
     assert t.dim() == 4 and t.shape == (B, n, heads, cache.head_dim), f'{what} must be [batch, tokens, heads, head_dim] with the head_dim of the cache'
     assert t.dtype == cache.dtype and t.device == cache.device, f'{what} must have the type and device of the cache'
-    return t if t.stride(3) == 1 else t.contiguous()
 
 
 def _no_grad(*ts):
@@ -139,37 +157,47 @@ def paged_append(cache, k, v, table, lengths, counts=None, rope=None, q=None, re
 
     Returns the rotated queries [B, n, heads, head_dim] (None without q); with return_keys, (queries, rotated keys [B, n, kv_heads, head_dim]): what the
     prompt's own attention takes.  Padding rows of both are zero.  Two rows of one call must not go to the same slot."""
-    assert k.dim() == 4, 'k must be [batch, tokens, heads, head_dim]'
-    B, n = k.shape[:2]
-    k, v = _rows(cache, k, B, n, cache.kv_heads, 'k'), _rows(cache, v, B, n, cache.kv_heads, 'v')
-    p = cache._params()
-    _places(p, cache, table, lengths, counts, B)
-    p.B, p.n = B, n
-    p.k, p.v = k.data_ptr(), v.data_ptr()
-    p.k_sb, p.k_sn, p.k_sh, _ = k.stride()
-    p.v_sb, p.v_sn, p.v_sh, _ = v.stride()
+    # rows that are not contiguous are copied, as in HyperAttention
+    k, v, q = [t if t is None or t.dim() == 0 or t.stride(-1) == 1 else t.contiguous() for t in (k, v, q)]
+    _no_grad(k, v) if q is None else _no_grad(k, v, q)
+
+    def make(p):
+        assert k.dim() == 4, 'k must be [batch, tokens, heads, head_dim]'
+        B, p.n = k.shape[:2]
+        _places(p, cache, table, lengths, counts, B)
+        _rows(cache, k, B, p.n, cache.kv_heads, 'k')
+        _rows(cache, v, B, p.n, cache.kv_heads, 'v')
+        p.k_sb, p.k_sn, p.k_sh, _ = k.stride()
+        p.v_sb, p.v_sn, p.v_sh, _ = v.stride()
+        if q is not None:
+            assert q.dim() == 4 and q.shape[2] % cache.kv_heads == 0, 'query heads must be a multiple of the key/value heads'
+            _rows(cache, q, B, p.n, q.shape[2], 'q')
+            p.H = q.shape[2]
+            p.q_sb, p.q_sn, p.q_sh, _ = q.stride()
+        if rope is not None:
+            assert rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous() and rope.device == cache.device, 'rope must be contiguous [positions, rot / 2, 2]'
+            assert rope.dtype in (torch.float32, cache.dtype) and 2 * rope.shape[1] <= cache.head_dim, \
+                'rope must be fp32 or of the cache\'s type, for at most head_dim elements'
+            p.rot, p.rope_rows, p.rope_dtype = 2 * rope.shape[1], rope.shape[0], ops._DT[rope.dtype]
+
+    cache._check_place()
+    raw, _ = cache._plan(('append', _form(k), _form(v), _form(q), _form(table), _form(lengths), _form(counts), _form(rope)), make)
+    p = L.PagedParams.from_buffer_copy(raw)
+    ops._set_status(p, cache.device)
+    p.k, p.v, p.table, p.lengths = k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr()
     q_out = k_out = None
+    if counts is not None:
+        p.counts = counts.data_ptr()
+    if rope is not None:
+        p.rope = rope.data_ptr()
     if q is not None:
-        assert q.dim() == 4 and q.shape[2] % cache.kv_heads == 0, 'query heads must be a multiple of the key/value heads'
-        q = _rows(cache, q, B, n, q.shape[2], 'q')
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        p.H, p.q, p.q_out = q.shape[2], q.data_ptr(), q_out.data_ptr()
-        p.q_sb, p.q_sn, p.q_sh, _ = q.stride()
-        _no_grad(k, v, q)
-    else:
-        _no_grad(k, v)
+        p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
     if return_keys:
         k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         p.k_out = k_out.data_ptr()
-    if rope is not None:
-        assert rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous() and rope.device == cache.device, 'rope must be contiguous [positions, rot / 2, 2]'
-        assert rope.dtype in (torch.float32, cache.dtype) and 2 * rope.shape[1] <= cache.head_dim, 'rope must be fp32 or of the cache\'s type, for at most head_dim elements'
-        p.rope, p.rot, p.rope_rows, p.rope_dtype = rope.data_ptr(), 2 * rope.shape[1], rope.shape[0], ops._DT[rope.dtype]
     L.check(ops._call(L.load().ha_paged_append, cache.device, C.byref(p)), 'ha_paged_append')
     return (q_out, k_out) if return_keys else q_out
-
-
-_WORKSPACE = {}         # bytes by sizes (bounded)
 
 
 def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
@@ -181,47 +209,62 @@ def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
     Row i < counts[b] sees positions 0 .. lengths[b] - counts[b] + i.  A row that sees none, and padding rows, have o = 0 and lse = -inf.  Consecutive
     query heads share a K/V head.  Every token reads the sequence's keys again (from the L2 cache where they fit): made for one to a few
     tokens a sequence; prompts belong to HyperAttention or flash_attn_func."""
-    assert q.dim() == 4 and q.shape[2] % cache.kv_heads == 0 and q.shape[2] > 0, 'q must be [batch, tokens, heads, head_dim], heads a multiple of the K/V heads'
-    B, n, H, d = q.shape
-    q = _rows(cache, q, B, n, H, 'q')
-    if (q.data_ptr() | (q.stride(0) | q.stride(1) | q.stride(2)) * 2) % 16:
-        q = q.contiguous() if q.data_ptr() % 16 == 0 and not q.is_contiguous() else q.clone(memory_format=torch.contiguous_format)
     _no_grad(q)
-    p = cache._params()
-    _places(p, cache, table, lengths, counts, B)
-    p.B, p.n, p.H = B, n, H
-    p.scale = float(softmax_scale or d ** -0.5)
-    p.q_sb, p.q_sn, p.q_sh, _ = q.stride()
-    o = torch.empty(B, n, H, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, n, dtype=torch.float32, device=q.device)
-    if not o.numel():
-        return o, lse
-    lib = L.load()
-    key = (cache.bits, B, n, H, cache.kv_heads, d, cache.page_size, p.columns, cache.device.index)
-    nbytes = _WORKSPACE.get(key)
-    if nbytes is None:
+    if q.dim() == 4 and (q.stride(3) != 1 or (q.data_ptr() | 2 * (q.stride(0) | q.stride(1) | q.stride(2))) % 16):
+        q = q.clone(memory_format=torch.contiguous_format)             # rows that the kernel's 16-byte loads cannot read
+    scale = float(softmax_scale or cache.head_dim ** -0.5)
+
+    def make(p):
+        assert q.dim() == 4 and q.shape[2] % cache.kv_heads == 0 and q.shape[2] > 0, 'q must be [batch, tokens, heads, head_dim], heads a multiple of the K/V heads'
+        B, p.n, p.H, _ = q.shape
+        _rows(cache, q, B, p.n, p.H, 'q')
+        _places(p, cache, table, lengths, counts, B)
+        p.q_sb, p.q_sn, p.q_sh, _ = q.stride()
+        p.scale = scale
+        lib = L.load()
         with torch.cuda.device(cache.device):
+            if cache.bits == 16 and cache._maps is None:
+                maps = C.create_string_buffer(256)
+                L.check(lib.ha_paged_maps(C.byref(p), maps), 'ha_paged_maps')
+                cache._maps = maps
+            p.maps = None if cache._maps is None else C.addressof(cache._maps)
             nbytes = lib.ha_paged_attn_workspace_bytes(C.byref(p))
-        if nbytes < 0:
-            L.check(nbytes, 'ha_paged_attn')
-        if len(_WORKSPACE) >= 512:
-            _WORKSPACE.clear()
-        _WORKSPACE[key] = nbytes
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    p.q, p.o, p.lse, p.workspace, p.workspace_bytes = q.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes
-    L.check(ops._call(lib.ha_paged_attn, cache.device, C.byref(p)), 'ha_paged_attn')
+        L.check(min(nbytes, 0), 'ha_paged_attn')
+        return nbytes, q.shape, (B, p.H, p.n)
+
+    cache._check_place()
+    raw, (nbytes, shape, lse_shape) = cache._plan(('attn', _form(q), _form(table), _form(lengths), _form(counts), scale), make)
+    dev = cache.device
+    o = torch.empty(shape, dtype=cache.dtype, device=dev)
+    lse = torch.empty(lse_shape, dtype=torch.float32, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    p = L.PagedParams.from_buffer_copy(raw)
+    ops._set_status(p, dev)
+    p.q, p.table, p.lengths, p.o, p.lse = q.data_ptr(), table.data_ptr(), lengths.data_ptr(), o.data_ptr(), lse.data_ptr()
+    p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+    if counts is not None:
+        p.counts = counts.data_ptr()
+    L.check(ops._call(L.load().ha_paged_attn, dev, C.byref(p)), 'ha_paged_attn')
     return o, lse
 
 
 def paged_gather(cache, table, lengths, rows):
     """Positions 0 .. rows - 1 of every sequence as dense (k, v) [B, kv_heads, rows, head_dim] in the cache's type, zero from lengths[b] (int32 [B]) on: the
     layout that HyperAttention takes."""
-    B = table.shape[0]
-    assert rows >= 0
-    p = cache._params()
-    _places(p, cache, table, lengths, None, B)
-    p.B, p.rows = B, rows
-    k, v = [torch.empty(B, cache.kv_heads, rows, cache.head_dim, dtype=cache.dtype, device=cache.device) for _ in 'kv']
-    p.k_out, p.v_out = k.data_ptr(), v.data_ptr()
+    rows = int(rows)
+
+    def make(p):
+        assert table.dim() == 2 and rows >= 0, 'table must be int32 [batch, columns], rows a number'
+        _places(p, cache, table, lengths, None, table.shape[0])
+        p.rows = rows
+        return table.shape[0], cache.kv_heads, rows, cache.head_dim
+
+    cache._check_place()
+    raw, shape = cache._plan(('gather', _form(table), _form(lengths), rows), make)
+    p = L.PagedParams.from_buffer_copy(raw)
+    ops._set_status(p, cache.device)
+    k = torch.empty(shape, dtype=cache.dtype, device=cache.device)
+    v = torch.empty(shape, dtype=cache.dtype, device=cache.device)
+    p.table, p.lengths, p.k_out, p.v_out = table.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr()
     L.check(ops._call(L.load().ha_paged_gather, cache.device, C.byref(p)), 'ha_paged_gather')
     return k, v

@@ -328,7 +328,13 @@ typedef struct ha_paged_params {
   void *workspace;
   int64_t workspace_bytes;
   int32_t *status, *status_host;
+  const void *maps;                       /* host memory, from ha_paged_maps; NULL: made in the call */
 } ha_paged_params;
+
+/* What ha_paged_attn needs to know about a 16-bit pool (HA_PAGED_MAPS_BYTES, the caller's), for a caller that keeps it beside the pool: making it anew
+ * costs a call a few microseconds of host time.  Depends on dtype, bits, Hk, d, pages, page_size, k_pages, v_pages and the page strides alone. */
+#define HA_PAGED_MAPS_BYTES 256
+int ha_paged_maps(const ha_paged_params* p, void* maps);
 
 /* Row i < counts[b] of k and v goes to position lengths[b] + i of sequence b, the first `rot` elements of k rotated there: pairs (2j, 2j+1),
  * (x0 c - x1 s, x1 c + x0 s), every product and sum rounded to 32 bits, the result once more to `dtype` (4 bits: the codes are taken from the 32-bit values).

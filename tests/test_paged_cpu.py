@@ -18,7 +18,7 @@ def lib():
 
 
 def test_struct_layout_matches_header():
-    assert C.sizeof(L.PagedParams) == 16 * 4 + 3 * 8 + 9 * 8 + 5 * 8 + 5 * 8 + 5 * 8 + 5 * 8 + 4 * 8
+    assert C.sizeof(L.PagedParams) == 16 * 4 + 3 * 8 + 9 * 8 + 5 * 8 + 5 * 8 + 5 * 8 + 5 * 8 + 5 * 8
 
 
 def _params(**over):
