@@ -57,14 +57,22 @@ inline PagedView paged_view(const ha_paged_params& p) {
   return v;
 }
 
-// Page and row within it of position `pos` (0 <= pos < capacity) of sequence b; page -1, and the failure reported, where the table names none.
-__device__ __forceinline__ int paged_slot(const PagedView& v, int b, int pos, int& row) {
+// The table's entry for position `pos` (0 <= pos < capacity) of sequence b, whatever it is, and the row within the page: the load alone, so that a kernel can
+// look ahead; paged_checked when the page is used.
+__device__ __forceinline__ int paged_entry(const PagedView& v, int b, int pos, int& row) {
   const int col = v.by_page(pos);
   row = pos - col * v.page_size;
-  const int page = v.table[b * v.table_sb + col];
-  if ((unsigned)page < (unsigned)v.pages) return page;
+  return v.table[b * v.table_sb + col];
+}
+__device__ __forceinline__ bool paged_checked(const PagedView& v, int page) {
+  if ((unsigned)page < (unsigned)v.pages) return true;
   report_status(v.status, v.status_host, HA_DEV_BAD_INDEX);
-  return -1;
+  return false;
+}
+// Page and row within it of position `pos` (0 <= pos < capacity) of sequence b; page -1, and the failure reported, where the table names none.
+__device__ __forceinline__ int paged_slot(const PagedView& v, int b, int pos, int& row) {
+  const int page = paged_entry(v, b, pos, row);
+  return paged_checked(v, page) ? page : -1;
 }
 
 }  // namespace ha

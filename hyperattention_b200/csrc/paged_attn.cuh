@@ -1,0 +1,249 @@
+// Shared by the attention kernels over the paged cache (16-bit and 4-bit rows).
+#pragma once
+#include "paged.cuh"
+#include "tensor_map.cuh"
+
+namespace ha {
+
+constexpr int attn4_tile(int d) { return d == 128 ? 128 : 256; }      // keys of a tile of 4-bit rows
+constexpr int ITEM_ROWS = 16;         // query heads of an item, at most
+constexpr int MAX_LINES = 256;        // (sequence, token) pairs of one launch: their tiles are summed up in shared memory
+// A weight's reference follows the running maximum only when that is 2^SLACK above it: with 16 rows a warp, some row's maximum grows at most of the first
+// dozens of tiles, and each time all the sums are scaled.  Weights, held in 16 bits for the products, have that much room above.
+constexpr float SLACK = 6.f;
+constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
+
+struct AttnArgs {
+  PagedView c;
+  const uint8_t* q;
+  int64_t q_sb, q_sn, q_sh;           // bytes
+  void* o;
+  float* lse;
+  int32_t n, H, Hk, group, blocks;    // blocks: items of a (token, K/V head): group / 16, rounded up
+  int32_t line0, lines;               // (sequence, token) pairs of this launch
+  int32_t run_log2;                   // rows that are fetched together: 2^run_log2, the largest power of two that pages and tiles are made of
+  int32_t whole_runs;                 // 4 bits: a warp's keys of a tile lie together, and their scales, on 16-byte boundaries
+  FastDiv by_n, by_blocks;
+  float scale_log2;                   // magnitude of the softmax scale, times log2 e
+  uint32_t flip;                      // sign bits of a pair of queries, where the scale is negative
+  float* part;                        // [CTAs][2][ITEM_ROWS][D], then ...
+  float2* part_stat;                  // [CTAs][2][ITEM_ROWS]: reference (log2), denominator
+  int4* head;                         // [CTAs]: last item's first and end tile, its line, its number
+  int32_t* meta;                      // all tiles, tiles of a CTA
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <int N>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, uint32_t src_bytes) {      // 4 or 8 bytes
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ uint2 lds64(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
+__device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
+// an arrival on `bar` once this thread's cp.async so far are done
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+// (a & mask) ^ flip in one instruction (of two constants the compiler would make two)
+__device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t mask, uint32_t flip) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(a), "r"(mask), "r"(flip));
+  return r;
+}
+__device__ __forceinline__ uint64_t dup_f2(float v) { return pack_f2(v, v); }
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+// A place in the list of tiles.
+struct Walk {
+  int line, item, tile, tiles;
+  __device__ __forceinline__ void settle(const int* first, int lines) {         // skips lines without keys
+    while (line < lines && (tiles = first[line + 1] - first[line]) == 0) ++line;
+  }
+  __device__ __forceinline__ void step(const int* first, int lines, int items) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++item < items) return;
+    item = 0;
+    ++line;
+    settle(first, lines);
+  }
+  __device__ __forceinline__ void skip(int by, const int* first, int lines, int items) {       // (the end of the list is by or more tiles away)
+    tile += by;
+    while (tile >= tiles) {
+      tile -= tiles;
+      if (++item < items) continue;
+      item = 0;
+      ++line;
+      settle(first, lines);
+    }
+  }
+};
+
+__device__ __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }      // 16-byte chunk of a query row in shared memory
+
+// Tiles before each line (of one item; first[lines]: all) and keys of each line, by the CTA's first 128 threads; every thread calls it.
+__device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int* first, int* keys, int* warp_sum) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int PER = (MAX_LINES + 1 + 127) / 128;
+  int before = 0, mine[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int line = tid * PER + u;
+    int m = 0;
+    if (line < a.lines) {
+      const int b = a.by_n(a.line0 + line), i = a.line0 + line - b * a.n;
+      const int count = a.c.counts ? min(a.c.counts[b], a.n) : a.n;
+      int len = a.c.lengths[b];
+      if (len > a.c.capacity) {
+        report_status(a.c.status, a.c.status_host, HA_DEV_BAD_INDEX);
+        len = a.c.capacity;
+      }
+      if (i < count) m = max(max(len, 0) - (count - 1 - i), 0);
+      keys[line] = m;
+    }
+    mine[u] = before;
+    before += (m + tile_keys - 1) / tile_keys;
+  }
+  int incl = before;
+#pragma unroll
+  for (int y = 1; y < 32; y *= 2) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, y);
+    if (lane >= y) incl += v;
+  }
+  if (lane == 31 && warp < 4) warp_sum[warp] = incl;
+  __syncthreads();
+  int ahead = incl - before;
+  for (int w = 0; w < min(warp, 4); ++w) ahead += warp_sum[w];
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    if (tid * PER + u <= a.lines) first[tid * PER + u] = ahead + mine[u];
+  __syncthreads();
+}
+
+// This CTA's part [begin, end) of the list of tiles, and the place of its first; lines without keys get their outputs here.
+template <typename T, int D>
+__device__ __forceinline__ Walk take_part(const AttnArgs& a, const int* first, const int* keys, int items, int& begin, int& end) {
+  const int tid = threadIdx.x;
+  const int total = first[a.lines] * items;
+  const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+  begin = min((int)blockIdx.x * per, total);
+  end = min(begin + per, total);
+  if (blockIdx.x == 0 && tid == 0) {
+    a.meta[0] = total;
+    a.meta[1] = per;
+  }
+  for (int line = blockIdx.x; line < a.lines; line += gridDim.x) {
+    if (keys[line] > 0) continue;
+    const int b = a.by_n(a.line0 + line), i = a.line0 + line - b * a.n;
+    uint4* o = reinterpret_cast<uint4*>((T*)a.o + (int64_t)(a.line0 + line) * a.H * D);
+    for (int e = tid; e < a.H * D / 8; e += blockDim.x) o[e] = make_uint4(0, 0, 0, 0);
+    for (int h = tid; h < a.H; h += blockDim.x) a.lse[((int64_t)b * a.H + h) * a.n + i] = -INFINITY;
+  }
+  Walk at = {a.lines, 0, 0, 1};
+  if (begin >= end) return at;
+  int lo = 0, hi = a.lines;                  // the last line whose tiles begin at or before `begin`
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] * items <= begin) lo = mid;
+    else hi = mid;
+  }
+  at.line = lo;
+  at.settle(first, a.lines);
+  const int off = begin - first[at.line] * items;
+  at.item = off / at.tiles;
+  at.tile = off - at.item * at.tiles;
+  return at;
+}
+
+// End of an item, or of this CTA's part of it: the sums of the four warps that compute are joined through `sums` (a stage that has been read), and go out as
+// the result or as a part.  `join`: all four warps are here and see what each wrote to shared memory; false: one gave up.
+template <typename T, int D, int APART, typename W, typename J>
+__device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* stat, float* sums, const Walk& at, const int* first, int items, int begin, int end,
+                                            bool last, J join) {
+  constexpr int ROWS = W::ROWS, ROUNDS = W::ROUNDS, WIDTH = D / ROUNDS, LANES = 128 / ROWS;     // threads of a row
+  static_assert(APART >= ROWS * WIDTH, "floats from one warp's sums to the next's");
+  static_assert(WIDTH % (4 * LANES) == 0, "whole columns");
+  const int tid = threadIdx.x, warp = tid >> 5;
+  w.statistics(stat + warp * ITEM_ROWS);
+  const int b = a.by_n(a.line0 + at.line), i = a.line0 + at.line - b * a.n;
+  const int h = a.by_blocks(at.item), block = at.item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
+  const int item_begin = first[at.line] * items + at.item * at.tiles, item_end = item_begin + at.tiles;
+  const bool whole = item_begin >= begin && item_end <= end;
+  const int row = tid / LANES;
+  const int64_t out = ((int64_t)(a.line0 + at.line) * a.H + h * a.group + block * ITEM_ROWS + row) * D;
+  const int slot = 2 * blockIdx.x + (item_begin <= begin ? 0 : 1);
+  float part[4], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int y = 0; y < ROUNDS; ++y) {
+    if (!join()) return false;               // the stage has been read (the round before, too); the statistics are there
+    w.put(sums + warp * APART, y);
+    if (y == 0) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) m = fmaxf(m, stat[x * ITEM_ROWS + row].x);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float2 st = stat[x * ITEM_ROWS + row];
+        part[x] = st.x == -INFINITY ? -1.f : fast_exp2(st.x - m);
+        if (!(part[x] < 0.f)) l = fmaf(part[x], st.y, l);
+      }
+    }
+    if (!join()) return false;
+    const float inv = whole ? 1.f / l : 1.f;
+#pragma unroll
+    for (int j = 0; j < WIDTH / (4 * LANES); ++j) {
+      const int col = (tid % LANES) * 4 + 4 * LANES * j;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float4 f = *reinterpret_cast<const float4*>(sums + x * APART + row * WIDTH + (col ^ W::turn(row)));
+        if (!(part[x] < 0.f)) {
+          v.x = fmaf(part[x], f.x, v.x);
+          v.y = fmaf(part[x], f.y, v.y);
+          v.z = fmaf(part[x], f.z, v.z);
+          v.w = fmaf(part[x], f.w, v.w);
+        }
+      }
+      if (row < rows) {
+        if (whole)
+          *reinterpret_cast<uint2*>((T*)a.o + out + y * WIDTH + col) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+        else
+          *reinterpret_cast<float4*>(a.part + ((int64_t)slot * ITEM_ROWS + row) * D + y * WIDTH + col) = v;
+      }
+    }
+    if (y == 0 && row < rows && tid % LANES == 0) {
+      if (whole) a.lse[((int64_t)b * a.H + h * a.group + block * ITEM_ROWS + row) * a.n + i] = (m + log2f(l)) * LN2;
+      else a.part_stat[slot * ITEM_ROWS + row] = make_float2(m, l);
+    }
+  }
+  if (last && tid == 0) a.head[blockIdx.x] = make_int4(item_begin, item_end, a.line0 + at.line, at.item);
+  return true;
+}
+
+// Kernels of 4-bit rows: CTAs of an SM, keys of a tile, and the launch of one kernel.
+int attn4_resident(int d, int group);
+int attn4_launch(AttnArgs a, int dtype, int d, int ctas, cudaStream_t st);
+
+}  // namespace ha
