@@ -54,6 +54,24 @@ inline void launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t s
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<A&&>(args)...);      // (its error is the one that HA_LAUNCHED finds)
 }
+// ... whose CTAs come in clusters of `cluster` neighbours.
+template <typename... P, typename... A>
+inline void launch_chained_clusters(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, A&&... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<A&&>(args)...);
+}
 // Lets the CTAs of a chained kernel that comes next be placed as soon as all of this kernel's are.
 __device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // First statement of every thread of a chained kernel: waits until the previous kernel is complete and its memory operations are visible.  Nothing is

@@ -26,6 +26,7 @@ namespace ha {
 namespace {
 
 constexpr int THREADS = 160;
+constexpr int CLUSTER_TILES = 10;     // tiles of a CTA, at most, where clusters share items
 
 template <int D>
 struct Stage {
@@ -37,6 +38,7 @@ struct Stage {
   static constexpr int BARS = 2 * NS + 1;
   static constexpr int SMEM = NS * BYTES + 4 * ITEM_ROWS * 8 + BARS * 8 + (2 * MAX_LINES + 8) * 4 + 16;
   static_assert(4 * ITEM_ROWS * D * 4 <= Q, "the warps' sums fit a stage");
+  static_assert(ITEM_ROWS * (D * 4 + 8) <= BYTES, "... and a cluster's part");
   static_assert(BYTES % 1024 == 0, "stages begin on the swizzle's boundary");
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs of an SM");
 };
@@ -187,18 +189,18 @@ struct Worker {
 };
 
 // The warp that fetches: tiles begin .. end - 1 into the ring.  full[s]: every lane arrives once its copies are there; empty[s]: the four warps that compute.
-template <int D>
+template <int D, bool CLUSTER>
 __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, const int* first, const int* keys, Walk at,
-                                            int begin, int end, int items, uint32_t base, uint32_t bars, int* abort_flag) {
+                                            int begin, int end, int items, int line0, uint32_t base, uint32_t bars, int* abort_flag) {
   using S = Stage<D>;
   constexpr int NS = S::NS, TK = S::TK;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, lines = CLUSTER ? 1 : a.lines;
   // page (not yet looked at) and slot of the run `r` of a tile; of one without keys: 0, and not to be used
   auto look_up = [&](const Walk& w, int r, int& slot) {
     slot = 0;
     const int key = w.tile * TK + (r << a.run_log2);
-    if (w.line >= a.lines || (r << a.run_log2) >= TK || key >= keys[w.line]) return 0;
-    return paged_entry(a.c, a.by_n(a.line0 + w.line), key, slot);
+    if (w.line >= lines || (r << a.run_log2) >= TK || key >= keys[w.line]) return 0;
+    return paged_entry(a.c, a.by_n(line0 + w.line), key, slot);
   };
   int slot, page = look_up(at, lane, slot);
   int s = 0;
@@ -207,11 +209,11 @@ __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap
     const uint32_t full = bars + 8 * s, empty = bars + 8 * (NS + s), dst = base + s * S::BYTES;
     if (round > 0 && !mbar_wait_or_abort(empty, (round - 1) & 1, abort_flag)) break;
     Walk next = at;
-    next.step(first, a.lines, items);
-    if (it + 1 == end) next.line = a.lines;
+    next.step(first, lines, items);
+    if (it + 1 == end) next.line = lines;
     int next_slot;
     const int next_page = look_up(next, lane, next_slot);              // (under way while this tile's copies are started)
-    const int b = a.by_n(a.line0 + at.line), i = a.line0 + at.line - b * a.n;
+    const int b = a.by_n(line0 + at.line), i = line0 + at.line - b * a.n;
     const int h = a.by_blocks(at.item), left = keys[at.line] - at.tile * TK;
     for (int r0 = 0; (r0 << a.run_log2) < min(TK, left); r0 += 32) {
       if (r0 > 0) page = look_up(at, r0 + lane, slot);                 // (runs of less than TK / 32 rows)
@@ -251,7 +253,7 @@ __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     paged_attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm) {
   using S = Stage<D>;
@@ -276,13 +278,19 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
   }
   // The kernel behind is let in at the end: its CTAs would take the places that come free one by one, several on some SMs and none on others
   // (1 x 131072 tokens, 32 heads x 64, passes back to back: 242 us with an early release, 165 without).
+  if (CLUSTER) chain_release();              // (short kernels, fewer CTAs than there is room for: the next one may be placed at once)
   chain_wait();
-  scan_lines(a, TK, first, keys, warp_sum);
-  int begin, end;
-  Walk at = take_part<T, D>(a, first, keys, items, begin, end);
-  if (begin >= end) return;
+  int begin, end, line0;
+  Walk at = take_part<T, D, CLUSTER>(a, TK, first, keys, warp_sum, items, begin, end, line0);
+  const int lines = CLUSTER ? 1 : a.lines, item = at.item;
+  if (begin >= end && (!CLUSTER || keys[0] == 0)) return;
   if (warp == 4) {
-    fetch_tiles<D>(a, &km, &vm, first, keys, at, begin, end, items, base, bars, abort_flag);
+    if (begin < end) fetch_tiles<D, CLUSTER>(a, &km, &vm, first, keys, at, begin, end, items, line0, base, bars, abort_flag);
+    if (CLUSTER) {                             // (these threads count in the cluster's barriers)
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
     return;
   }
 
@@ -294,6 +302,9 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     if (lane == 0) mbar_arrive(join_bar);
     return mbar_wait_or_abort(join_bar, joined++ & 1, abort_flag);
   };
+  // with clusters: this CTA's part, in the same place of every CTA (no stage is used any more when it is written)
+  float* cluster_sums = reinterpret_cast<float*>(smem);
+  float2* cluster_stat = reinterpret_cast<float2*>(cluster_sums + ITEM_ROWS * D);
   int s = 0;
   uint32_t round = 0;
   bool ok = true;
@@ -308,15 +319,22 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     w.tile(stage, left, a.scale_log2);
     const bool ends = at.tile == at.tiles - 1 || it == end - 1;
     if (ends) {
-      ok = finish_item<T, D, 16 * D>(a, w, stat, reinterpret_cast<float*>(stage), at, first, items, begin, end, it == end - 1, join);
+      ok = finish_item<T, D, 16 * D, CLUSTER>(a, w, stat, reinterpret_cast<float*>(stage), at, first, items, begin, end, it == end - 1, line0, cluster_sums, cluster_stat, join);
       if (!ok) break;
     }
     // the stage is free (what was written to it by stores before what copies write to it next)
     if (ends || left < S::KW) fence_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(bars + 8 * (NS + s));
-    at.step(first, a.lines, items);
+    at.step(first, lines, items);
     if (++s == NS) s = 0, ++round;
+  }
+  if constexpr (CLUSTER) {
+    if (begin >= end || !ok) {
+      if (tid < ITEM_ROWS) cluster_stat[tid] = make_float2(-INFINITY, 0.f);
+    }
+    __syncwarp();
+    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, item);
   }
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   chain_release();
@@ -393,6 +411,18 @@ int attn_ctas(const ha_paged_params& p, int lines) {
   return (int)(most < 1 ? 1 : most < resident ? most : resident);
 }
 
+// CTAs that share an item as a cluster, or 0.  Short contexts and few items: a cluster joins its parts over distributed shared memory, without a workspace and a
+// second launch (1 x 515 tokens: 8.1 -> 5.5 us on the device, 7 -> 4 us of host time).  Every item gets the same CTAs, however long it is, so that the list of tiles,
+// which deals them out evenly, is for what takes longer than the joining.
+int attn_cluster(const ha_paged_params& p) {
+  const int64_t units = (int64_t)p.B * p.n * p.Hk * ((p.H / p.Hk + ITEM_ROWS - 1) / ITEM_ROWS);
+  const int64_t tiles = ((int64_t)p.columns * p.page_size + attn_tile(p) - 1) / attn_tile(p), resident = (int64_t)sm_count() * attn_resident(p);
+  if (units > resident || tiles == 0) return 0;
+  int c = 1;
+  while (c < 8 && c < tiles && units * 2 * c <= resident) c *= 2;
+  return (tiles + c - 1) / c <= CLUSTER_TILES ? c : 0;
+}
+
 // Lines of one launch: no more than shared memory counts, their tiles within 31 bits.
 int64_t attn_lines(const ha_paged_params& p) {
   const int tk = attn_tile(p), items = p.Hk * ((p.H / p.Hk + ITEM_ROWS - 1) / ITEM_ROWS);
@@ -419,8 +449,13 @@ int launch_attn(const AttnArgs& a, const ha_paged_params& p, int ctas, cudaStrea
   CUtensorMap maps[2] = {};
   if (p.maps) memcpy(maps, p.maps, sizeof(maps));
   else if (!attn_maps(p, maps)) return HA_ERR_INVALID;
-  HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D>), S::SMEM, "ha_paged_attn");
-  launch_chained(paged_attn_kernel<T, D>, ctas, THREADS, S::SMEM, st, a, maps[0], maps[1]);
+  if (a.cluster > 0) {
+    HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D, true>), S::SMEM, "ha_paged_attn");
+    launch_chained_clusters(paged_attn_kernel<T, D, true>, ctas, THREADS, S::SMEM, a.cluster, st, a, maps[0], maps[1]);
+  } else {
+    HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D, false>), S::SMEM, "ha_paged_attn");
+    launch_chained(paged_attn_kernel<T, D, false>, ctas, THREADS, S::SMEM, st, a, maps[0], maps[1]);
+  }
   HA_LAUNCHED("ha_paged_attn");
   return HA_OK;
 }
@@ -462,7 +497,7 @@ int64_t ha_paged_attn_workspace_bytes(const ha_paged_params* pp) {
     return HA_ERR_INVALID;
   if ((int64_t)p.columns * p.page_size > 0x7fffffffLL) return HA_ERR_TOO_LARGE;
   const int64_t all = (int64_t)p.B * p.n, lines = attn_lines(p);
-  if (all == 0) return 0;
+  if (all == 0 || attn_cluster(p) > 0) return 0;
   return lines < 1 ? (int64_t)HA_ERR_TOO_LARGE : attn_workspace(p, attn_ctas(p, (int)lines));
 }
 
@@ -474,7 +509,8 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   if (p.B == 0 || p.n == 0) return HA_OK;
   if (!p.q || !p.o || !p.lse || ((uintptr_t)p.q | (uintptr_t)p.o) % 16 != 0 || (p.q_sb | p.q_sn | p.q_sh) % 8 != 0) return HA_ERR_INVALID;
   const int ctas = attn_ctas(p, (int)attn_lines(p));
-  if (!p.workspace || (uintptr_t)p.workspace % 16 != 0 || p.workspace_bytes < attn_workspace(p, ctas)) return HA_ERR_WORKSPACE;
+  const int cluster = attn_cluster(p);
+  if (cluster == 0 && (!p.workspace || (uintptr_t)p.workspace % 16 != 0 || p.workspace_bytes < attn_workspace(p, ctas))) return HA_ERR_WORKSPACE;
   AttnArgs a = {};
   a.c = paged_view(p);
   a.q = (const uint8_t*)p.q;
@@ -484,6 +520,7 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   a.by_n = FastDiv((uint32_t)p.n); a.by_blocks = FastDiv((uint32_t)a.blocks);
   a.scale_log2 = fabsf(p.scale) * LOG2E;
   a.flip = p.scale < 0.f ? 0x80008000u : 0u;
+  a.cluster = cluster;
   uint8_t* ws = (uint8_t*)p.workspace;
   a.meta = (int32_t*)ws;
   a.head = (int4*)(ws + 256);
@@ -498,17 +535,17 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   }
   const cudaStream_t st = (cudaStream_t)stream;
   const bool bf = p.dtype == HA_BF16;
-  const int64_t all = (int64_t)p.B * p.n, most = attn_lines(p);
+  const int64_t all = (int64_t)p.B * p.n, most = cluster > 0 ? all : attn_lines(p);
   for (int64_t line0 = 0; line0 < all; line0 += most) {
     a.line0 = (int)line0;
     a.lines = (int)(all - line0 < most ? all - line0 : most);
-    const int now = attn_ctas(p, a.lines);
+    const int now = cluster > 0 ? a.lines * p.Hk * a.blocks * cluster : attn_ctas(p, a.lines);
     int rc;
     if (p.bits == 4) rc = attn4_launch(a, p.dtype, p.d, now, st);
     else if (p.d == 64) rc = bf ? launch_attn<__nv_bfloat16, 64>(a, p, now, st) : launch_attn<__half, 64>(a, p, now, st);
     else rc = bf ? launch_attn<__nv_bfloat16, 128>(a, p, now, st) : launch_attn<__half, 128>(a, p, now, st);
     if (rc != HA_OK) return rc;
-    if (now == 1) continue;
+    if (now == 1 || cluster > 0) continue;
     const dim3 grid(now - 1, a.group < ITEM_ROWS ? a.group : ITEM_ROWS);
     if (p.d == 64) {
       if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 64>, grid, 128, 0, st, a);

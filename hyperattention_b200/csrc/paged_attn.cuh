@@ -21,6 +21,7 @@ struct AttnArgs {
   float* lse;
   int32_t n, H, Hk, group, blocks;    // blocks: items of a (token, K/V head): group / 16, rounded up
   int32_t line0, lines;               // (sequence, token) pairs of this launch
+  int32_t cluster;                    // CTAs that share an item, a cluster of them; 0: the list of tiles
   int32_t run_log2;                   // rows that are fetched together: 2^run_log2, the largest power of two that pages and tiles are made of
   int32_t whole_runs;                 // 4 bits: a warp's keys of a tile lie together, and their scales, on 16-byte boundaries
   FastDiv by_n, by_blocks;
@@ -104,6 +105,18 @@ struct Walk {
 
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }      // 16-byte chunk of a query row in shared memory
 
+// Keys that a line (a token of a sequence) sees.
+__device__ __forceinline__ int keys_of(const AttnArgs& a, int line) {
+  const int b = a.by_n(line), i = line - b * a.n;
+  const int count = a.c.counts ? min(a.c.counts[b], a.n) : a.n;
+  int len = a.c.lengths[b];
+  if (len > a.c.capacity) {
+    report_status(a.c.status, a.c.status_host, HA_DEV_BAD_INDEX);
+    len = a.c.capacity;
+  }
+  return i < count ? max(max(len, 0) - (count - 1 - i), 0) : 0;
+}
+
 // Tiles before each line (of one item; first[lines]: all) and keys of each line, by the CTA's first 128 threads; every thread calls it.
 __device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int* first, int* keys, int* warp_sum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -113,17 +126,7 @@ __device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int
   for (int u = 0; u < PER; ++u) {
     const int line = tid * PER + u;
     int m = 0;
-    if (line < a.lines) {
-      const int b = a.by_n(a.line0 + line), i = a.line0 + line - b * a.n;
-      const int count = a.c.counts ? min(a.c.counts[b], a.n) : a.n;
-      int len = a.c.lengths[b];
-      if (len > a.c.capacity) {
-        report_status(a.c.status, a.c.status_host, HA_DEV_BAD_INDEX);
-        len = a.c.capacity;
-      }
-      if (i < count) m = max(max(len, 0) - (count - 1 - i), 0);
-      keys[line] = m;
-    }
+    if (line < a.lines) keys[line] = m = keys_of(a, a.line0 + line);
     mine[u] = before;
     before += (m + tile_keys - 1) / tile_keys;
   }
@@ -143,57 +146,80 @@ __device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int
   __syncthreads();
 }
 
-// This CTA's part [begin, end) of the list of tiles, and the place of its first; lines without keys get their outputs here.
 template <typename T, int D>
-__device__ __forceinline__ Walk take_part(const AttnArgs& a, const int* first, const int* keys, int items, int& begin, int& end) {
+__device__ __forceinline__ void empty_line(const AttnArgs& a, int line) {
+  const int b = a.by_n(line), i = line - b * a.n;
+  uint4* o = reinterpret_cast<uint4*>((T*)a.o + (int64_t)line * a.H * D);
+  for (int e = threadIdx.x; e < a.H * D / 8; e += blockDim.x) o[e] = make_uint4(0, 0, 0, 0);
+  for (int h = threadIdx.x; h < a.H; h += blockDim.x) a.lse[((int64_t)b * a.H + h) * a.n + i] = -INFINITY;
+}
+
+// This CTA's part [begin, end) of the list of tiles, and the place of its first; lines without keys get their outputs here.  With clusters, its part of
+// one item's tiles: line 0 of what it sees, which is line `line0` of the call.  Every thread calls it.
+template <typename T, int D, bool CLUSTER>
+__device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int* first, int* keys, int* warp_sum, int items, int& begin, int& end, int& line0) {
   const int tid = threadIdx.x;
-  const int total = first[a.lines] * items;
-  const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
-  begin = min((int)blockIdx.x * per, total);
-  end = min(begin + per, total);
-  if (blockIdx.x == 0 && tid == 0) {
-    a.meta[0] = total;
-    a.meta[1] = per;
+  if constexpr (CLUSTER) {
+    const int unit = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster, line = unit / items;
+    line0 = line;
+    const int m = keys_of(a, line), tiles = (m + tile_keys - 1) / tile_keys, share = (tiles + a.cluster - 1) / a.cluster;
+    if (tid == 0) {
+      first[0] = 0;
+      first[1] = tiles;
+      keys[0] = m;
+    }
+    __syncthreads();
+    begin = min(rank * share, tiles);
+    end = min(begin + share, tiles);
+    if (m == 0 && rank == 0 && unit % items == 0) empty_line<T, D>(a, line);
+    return Walk{0, unit % items, begin, tiles};
+  } else {
+    line0 = a.line0;
+    scan_lines(a, tile_keys, first, keys, warp_sum);
+    const int total = first[a.lines] * items;
+    const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+    begin = min((int)blockIdx.x * per, total);
+    end = min(begin + per, total);
+    if (blockIdx.x == 0 && tid == 0) {
+      a.meta[0] = total;
+      a.meta[1] = per;
+    }
+    for (int line = blockIdx.x; line < a.lines; line += gridDim.x) {
+      if (keys[line] == 0) empty_line<T, D>(a, a.line0 + line);
+    }
+    Walk at = {a.lines, 0, 0, 1};
+    if (begin >= end) return at;
+    int lo = 0, hi = a.lines;                  // the last line whose tiles begin at or before `begin`
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (first[mid] * items <= begin) lo = mid;
+      else hi = mid;
+    }
+    at.line = lo;
+    at.settle(first, a.lines);
+    const int off = begin - first[at.line] * items;
+    at.item = off / at.tiles;
+    at.tile = off - at.item * at.tiles;
+    return at;
   }
-  for (int line = blockIdx.x; line < a.lines; line += gridDim.x) {
-    if (keys[line] > 0) continue;
-    const int b = a.by_n(a.line0 + line), i = a.line0 + line - b * a.n;
-    uint4* o = reinterpret_cast<uint4*>((T*)a.o + (int64_t)(a.line0 + line) * a.H * D);
-    for (int e = tid; e < a.H * D / 8; e += blockDim.x) o[e] = make_uint4(0, 0, 0, 0);
-    for (int h = tid; h < a.H; h += blockDim.x) a.lse[((int64_t)b * a.H + h) * a.n + i] = -INFINITY;
-  }
-  Walk at = {a.lines, 0, 0, 1};
-  if (begin >= end) return at;
-  int lo = 0, hi = a.lines;                  // the last line whose tiles begin at or before `begin`
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (first[mid] * items <= begin) lo = mid;
-    else hi = mid;
-  }
-  at.line = lo;
-  at.settle(first, a.lines);
-  const int off = begin - first[at.line] * items;
-  at.item = off / at.tiles;
-  at.tile = off - at.item * at.tiles;
-  return at;
 }
 
 // End of an item, or of this CTA's part of it: the sums of the four warps that compute are joined through `sums` (a stage that has been read), and go out as
 // the result or as a part.  `join`: all four warps are here and see what each wrote to shared memory; false: one gave up.
-template <typename T, int D, int APART, typename W, typename J>
+template <typename T, int D, int APART, bool CLUSTER, typename W, typename J>
 __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* stat, float* sums, const Walk& at, const int* first, int items, int begin, int end,
-                                            bool last, J join) {
+                                            bool last, int line0, float* cluster_sums, float2* cluster_stat, J join) {
   constexpr int ROWS = W::ROWS, ROUNDS = W::ROUNDS, WIDTH = D / ROUNDS, LANES = 128 / ROWS;     // threads of a row
   static_assert(APART >= ROWS * WIDTH, "floats from one warp's sums to the next's");
   static_assert(WIDTH % (4 * LANES) == 0, "whole columns");
   const int tid = threadIdx.x, warp = tid >> 5;
   w.statistics(stat + warp * ITEM_ROWS);
-  const int b = a.by_n(a.line0 + at.line), i = a.line0 + at.line - b * a.n;
+  const int b = a.by_n(line0 + at.line), i = line0 + at.line - b * a.n;
   const int h = a.by_blocks(at.item), block = at.item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
   const int item_begin = first[at.line] * items + at.item * at.tiles, item_end = item_begin + at.tiles;
-  const bool whole = item_begin >= begin && item_end <= end;
+  const bool whole = !CLUSTER && item_begin >= begin && item_end <= end;
   const int row = tid / LANES;
-  const int64_t out = ((int64_t)(a.line0 + at.line) * a.H + h * a.group + block * ITEM_ROWS + row) * D;
+  const int64_t out = ((int64_t)(line0 + at.line) * a.H + h * a.group + block * ITEM_ROWS + row) * D;
   const int slot = 2 * blockIdx.x + (item_begin <= begin ? 0 : 1);
   float part[4], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -212,10 +238,12 @@ __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* sta
     }
     if (!join()) return false;
     const float inv = whole ? 1.f / l : 1.f;
+    float4 vs[WIDTH / (4 * LANES)];
 #pragma unroll
     for (int j = 0; j < WIDTH / (4 * LANES); ++j) {
       const int col = (tid % LANES) * 4 + 4 * LANES * j;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4& v = vs[j];
+      v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float4 f = *reinterpret_cast<const float4*>(sums + x * APART + row * WIDTH + (col ^ W::turn(row)));
@@ -226,20 +254,82 @@ __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* sta
           v.w = fmaf(part[x], f.w, v.w);
         }
       }
-      if (row < rows) {
+    }
+    // (a cluster's part may lie where the sums did)
+    if (CLUSTER && !join()) return false;
+    if (row < rows) {
+#pragma unroll
+      for (int j = 0; j < WIDTH / (4 * LANES); ++j) {
+        const int col = (tid % LANES) * 4 + 4 * LANES * j;
+        const float4 v = vs[j];
         if (whole)
           *reinterpret_cast<uint2*>((T*)a.o + out + y * WIDTH + col) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+        else if (CLUSTER)
+          *reinterpret_cast<float4*>(cluster_sums + row * D + y * WIDTH + col) = v;
         else
           *reinterpret_cast<float4*>(a.part + ((int64_t)slot * ITEM_ROWS + row) * D + y * WIDTH + col) = v;
       }
     }
     if (y == 0 && row < rows && tid % LANES == 0) {
       if (whole) a.lse[((int64_t)b * a.H + h * a.group + block * ITEM_ROWS + row) * a.n + i] = (m + log2f(l)) * LN2;
+      else if (CLUSTER) cluster_stat[row] = make_float2(m, l);
       else a.part_stat[slot * ITEM_ROWS + row] = make_float2(m, l);
     }
   }
-  if (last && tid == 0) a.head[blockIdx.x] = make_int4(item_begin, item_end, a.line0 + at.line, at.item);
+  if (last && !CLUSTER && tid == 0) a.head[blockIdx.x] = make_int4(item_begin, item_end, a.line0 + at.line, at.item);
   return true;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+
+// End of an item that a cluster shares: each CTA joins its share of the rows from all CTAs' parts, read over distributed shared memory.  The first four warps of every
+// CTA call it, those of a CTA without keys, too (stat -inf); no CTA leaves before the others have read its part.
+template <typename T, int D>
+__device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* sums, const float2* stat, int line, int item) {
+  cluster_sync();
+  const int tid = threadIdx.x, rank = blockIdx.x % a.cluster;
+  const int b = a.by_n(line), i = line - b * a.n;
+  const int h = a.by_blocks(item), block = item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
+  constexpr int LANES = D / 4;                 // threads of a row, four columns each
+  for (int row = rank + a.cluster * (tid / LANES); row < rows; row += a.cluster * (128 / LANES)) {
+    const int col = tid % LANES * 4;
+    float m = -INFINITY, l = 0.f;
+    float2 st[8];
+    float4 f[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      st[x] = make_float2(-INFINITY, 0.f);
+      if (x >= a.cluster) continue;
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(st[x].x), "=f"(st[x].y) : "r"(cluster_at(stat + row, x)));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[x].x), "=f"(f[x].y), "=f"(f[x].z), "=f"(f[x].w) : "r"(cluster_at(sums + row * D + col, x)));
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) m = fmaxf(m, st[x].x);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      if (st[x].x == -INFINITY) continue;
+      const float w = fast_exp2(st[x].x - m);
+      l = fmaf(w, st[x].y, l);
+      v.x = fmaf(w, f[x].x, v.x);
+      v.y = fmaf(w, f[x].y, v.y);
+      v.z = fmaf(w, f[x].z, v.z);
+      v.w = fmaf(w, f[x].w, v.w);
+    }
+    const float inv = 1.f / l;
+    const int head = h * a.group + block * ITEM_ROWS + row;
+    *reinterpret_cast<uint2*>((T*)a.o + ((int64_t)line * a.H + head) * D + col) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+    if (col == 0) a.lse[((int64_t)b * a.H + head) * a.n + i] = (m + log2f(l)) * LN2;
+  }
+  cluster_sync();
 }
 
 // Kernels of 4-bit rows: CTAs of an SM, keys of a tile, and the launch of one kernel.

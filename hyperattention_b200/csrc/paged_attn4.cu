@@ -28,7 +28,8 @@ struct Stage4 {
   static constexpr int CTAS = D == 128 ? 3 : 4, NS = 2;
   static constexpr int QF = (NQ == 2 ? D * 32 : 0) + (1 + G) * ROWS * 4;   // a warp's query operands (16 rows); units and sums of the queries
   static constexpr int WARP = NS * BYTES + QF + NS * 16 + 64;          // of a warp, too: what its stages hold, and its place in the list
-  static constexpr int SMEM = 4 * WARP + 4 * ITEM_ROWS * 8 + (2 * MAX_LINES + 8) * 4 + 32;
+  static constexpr int PARTS = ROWS * (D * 4 + 8);           // with clusters: the CTA's part
+  static constexpr int SMEM = 4 * WARP + PARTS + 4 * ITEM_ROWS * 8 + (2 * MAX_LINES + 8) * 4 + 32;
   static constexpr int ROUNDS = NQ;                          // in which the warps' sums are joined: column ranges that fit a stage
   static_assert(ROWS * D / ROUNDS * 4 <= BYTES, "a warp's sums fit a stage");
   static_assert(WK * ROW == 2048 && WK * SC == 256 && WARP % 16 == 0, "copies of a warp's rows and scales");
@@ -417,12 +418,14 @@ struct alignas(16) Place {
   int keys;
 };
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, bool CLUSTER>
 __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel(const __grid_constant__ AttnArgs a) {
   using S = Stage4<D, NQ>;
   constexpr int NS = S::NS, TK = S::TK, KW = S::KW, WK = S::WK;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float2* stat = reinterpret_cast<float2*>(smem + 4 * S::WARP);              // [4][ITEM_ROWS]
+  float* cluster_sums = reinterpret_cast<float*>(smem + 4 * S::WARP);        // [ROWS][D]
+  float2* cluster_stat = reinterpret_cast<float2*>(cluster_sums + S::ROWS * D);
+  float2* stat = cluster_stat + S::ROWS;                                     // [4][ITEM_ROWS]
   int* first = reinterpret_cast<int*>(stat + 4 * ITEM_ROWS);                 // [lines + 1]
   int* abort_flag = first + MAX_LINES + 3;
   int* keys = first + MAX_LINES + 4;                                         // [lines]
@@ -435,11 +438,12 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     mbar_fence_init();
     *abort_flag = 0;
   }
-  chain_wait();                                // (the kernel behind is let in at the end, as in paged_attn.cu)
-  scan_lines(a, TK, first, keys, warp_sum);
-  int begin, end;
-  const Walk start = take_part<T, D>(a, first, keys, items, begin, end);
-  if (begin >= end) return;
+  if (CLUSTER) chain_release();              // (as in paged_attn.cu: the kernel behind is let in at the end, or at once)
+  chain_wait();
+  int begin, end, line0;
+  const Walk start = take_part<T, D, CLUSTER>(a, TK, first, keys, warp_sum, items, begin, end, line0);
+  const int lines = CLUSTER ? 1 : a.lines;
+  if (begin >= end && (!CLUSTER || keys[0] == 0)) return;
 
   uint8_t* mine = smem + warp * S::WARP;                                     // stages, query operands, what the stages hold
   int4* what = reinterpret_cast<int4*>(mine + NS * S::BYTES + S::QF);
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
   const uint32_t base = smem_u32(mine);
   auto settle = [&](const Walk& f) {
     const int h = a.by_blocks(f.item);
-    place->table = a.c.table + a.by_n(a.line0 + f.line) * a.c.table_sb;
+    place->table = a.c.table + a.by_n(line0 + f.line) * a.c.table_sb;
     place->head = h * a.c.sh;
     place->head_s = h * a.c.ssh;
     place->keys = keys[f.line];
@@ -502,9 +506,9 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
         place->tile = f.tile + 1;
       } else {
         Walk next = {f.line, f.item, f.tile, f.tiles};
-        next.step(first, a.lines, items);
+        next.step(first, lines, items);
         place->line = next.line, place->item = next.item, place->tile = next.tile, place->tiles = next.tiles;
-        if (next.line < a.lines) settle(next);
+        if (next.line < lines) settle(next);
       }
     }
     __syncwarp();
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     __syncwarp();
     const int4 t = what[s];
     if (it == begin || t.w == 0) {
-      const int b = a.by_n(a.line0 + t.y), i = a.line0 + t.y - b * a.n, h = a.by_blocks(t.z), block = t.z - h * a.blocks;
+      const int b = a.by_n(line0 + t.y), i = line0 + t.y - b * a.n, h = a.by_blocks(t.z), block = t.z - h * a.blocks;
       w.begin(a, a.q + b * a.q_sb + i * a.q_sn + (int64_t)(h * a.group + block * ITEM_ROWS) * a.q_sh, min(a.group - block * ITEM_ROWS, ITEM_ROWS));
     }
     if (t.x < WK) w.clear_tail(stage, t.x);
@@ -550,13 +554,20 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     for (int y = 0; y < WK; y += KW) w.keys(stage, y, t.x - y);
     if (t.x + warp * WK <= TK || it == end - 1) {
       const Walk at = {t.y, t.z, t.w, first[t.y + 1] - first[t.y]};
-      ok = finish_item<T, D, S::WARP / 4>(a, w, stat, reinterpret_cast<float*>(smem + s * S::BYTES), at, first, items, begin, end, it == end - 1, join) && join();
+      ok = finish_item<T, D, S::WARP / 4, CLUSTER>(a, w, stat, reinterpret_cast<float*>(smem + s * S::BYTES), at, first, items, begin, end, it == end - 1, line0, cluster_sums, cluster_stat, join) && join();
       if (!ok) break;
     }
     __syncwarp();
     if (it + NS < end) fetch(s);
     cp_async_commit();
     if (++s == NS) s = 0;
+  }
+  if constexpr (CLUSTER) {
+    if (begin >= end || !ok) {
+      if (tid < S::ROWS) cluster_stat[tid] = make_float2(-INFINITY, 0.f);
+    }
+    __syncwarp();
+    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, start.item);
   }
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   cp_async_wait<0>();
@@ -566,8 +577,13 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
 template <typename T, int D, int NQ>
 int launch4(const AttnArgs& a, int ctas, cudaStream_t st) {
   using S = Stage4<D, NQ>;
-  HA_SMEM_ATTR_ONCE((paged_attn4_kernel<T, D, NQ>), S::SMEM, "ha_paged_attn");
-  launch_chained(paged_attn4_kernel<T, D, NQ>, ctas, 128, S::SMEM, st, a);
+  if (a.cluster > 0) {
+    HA_SMEM_ATTR_ONCE((paged_attn4_kernel<T, D, NQ, true>), S::SMEM, "ha_paged_attn");
+    launch_chained_clusters(paged_attn4_kernel<T, D, NQ, true>, ctas, 128, S::SMEM, a.cluster, st, a);
+  } else {
+    HA_SMEM_ATTR_ONCE((paged_attn4_kernel<T, D, NQ, false>), S::SMEM, "ha_paged_attn");
+    launch_chained(paged_attn4_kernel<T, D, NQ, false>, ctas, 128, S::SMEM, st, a);
+  }
   HA_LAUNCHED("ha_paged_attn");
   return HA_OK;
 }

@@ -123,6 +123,19 @@ def _form(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
+# (an allocation of known strides costs a third less host time than torch.empty, and these calls are that time where the batch is small)
+_new = torch.empty_strided
+
+
+def _dense(*shape):
+    """Sizes and strides of a contiguous tensor."""
+    strides, n = [], 1
+    for s in reversed(shape):
+        strides.append(n)
+        n *= max(s, 1)
+    return shape, tuple(reversed(strides))
+
+
 def _places(p, cache, table, lengths, counts, B):
     """Checks the table and the lengths of a call, and fills in their sizes."""
     ops._cuda(cache.k)
@@ -179,9 +192,10 @@ def paged_append(cache, k, v, table, lengths, counts=None, rope=None, q=None, re
             assert rope.dtype in (torch.float32, cache.dtype) and 2 * rope.shape[1] <= cache.head_dim, \
                 'rope must be fp32 or of the cache\'s type, for at most head_dim elements'
             p.rot, p.rope_rows, p.rope_dtype = 2 * rope.shape[1], rope.shape[0], ops._DT[rope.dtype]
+        return _dense(*k.shape), None if q is None else _dense(*q.shape)
 
     cache._check_place()
-    raw, _ = cache._plan(('append', _form(k), _form(v), _form(q), _form(table), _form(lengths), _form(counts), _form(rope)), make)
+    raw, (k_form, q_form) = cache._plan(('append', _form(k), _form(v), _form(q), _form(table), _form(lengths), _form(counts), _form(rope)), make)
     p = L.PagedParams.from_buffer_copy(raw)
     ops._set_status(p, cache.device)
     p.k, p.v, p.table, p.lengths = k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr()
@@ -191,10 +205,10 @@ def paged_append(cache, k, v, table, lengths, counts=None, rope=None, q=None, re
     if rope is not None:
         p.rope = rope.data_ptr()
     if q is not None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = _new(*q_form, dtype=cache.dtype, device=cache.device)
         p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
     if return_keys:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_out = _new(*k_form, dtype=cache.dtype, device=cache.device)
         p.k_out = k_out.data_ptr()
     L.check(ops._call(L.load().ha_paged_append, cache.device, C.byref(p)), 'ha_paged_append')
     return (q_out, k_out) if return_keys else q_out
@@ -230,18 +244,19 @@ def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
             p.maps = None if cache._maps is None else C.addressof(cache._maps)
             nbytes = lib.ha_paged_attn_workspace_bytes(C.byref(p))
         L.check(min(nbytes, 0), 'ha_paged_attn')
-        return nbytes, q.shape, (B, p.H, p.n)
+        return nbytes, _dense(*q.shape), _dense(B, p.H, p.n)
 
     cache._check_place()
-    raw, (nbytes, shape, lse_shape) = cache._plan(('attn', _form(q), _form(table), _form(lengths), _form(counts), scale), make)
+    raw, (nbytes, form, lse_form) = cache._plan(('attn', _form(q), _form(table), _form(lengths), _form(counts), scale), make)
     dev = cache.device
-    o = torch.empty(shape, dtype=cache.dtype, device=dev)
-    lse = torch.empty(lse_shape, dtype=torch.float32, device=dev)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    o = _new(*form, dtype=cache.dtype, device=dev)
+    lse = _new(*lse_form, dtype=torch.float32, device=dev)
     p = L.PagedParams.from_buffer_copy(raw)
     ops._set_status(p, dev)
     p.q, p.table, p.lengths, p.o, p.lse = q.data_ptr(), table.data_ptr(), lengths.data_ptr(), o.data_ptr(), lse.data_ptr()
-    p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+    if nbytes:
+        ws = _new((nbytes,), (1,), dtype=torch.uint8, device=dev)        # (free once the launches are enqueued: same stream)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
     if counts is not None:
         p.counts = counts.data_ptr()
     L.check(ops._call(L.load().ha_paged_attn, dev, C.byref(p)), 'ha_paged_attn')
@@ -257,14 +272,14 @@ def paged_gather(cache, table, lengths, rows):
         assert table.dim() == 2 and rows >= 0, 'table must be int32 [batch, columns], rows a number'
         _places(p, cache, table, lengths, None, table.shape[0])
         p.rows = rows
-        return table.shape[0], cache.kv_heads, rows, cache.head_dim
+        return _dense(table.shape[0], cache.kv_heads, rows, cache.head_dim)
 
     cache._check_place()
-    raw, shape = cache._plan(('gather', _form(table), _form(lengths), rows), make)
+    raw, form = cache._plan(('gather', _form(table), _form(lengths), rows), make)
     p = L.PagedParams.from_buffer_copy(raw)
     ops._set_status(p, cache.device)
-    k = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-    v = torch.empty(shape, dtype=cache.dtype, device=cache.device)
+    k = _new(*form, dtype=cache.dtype, device=cache.device)
+    v = _new(*form, dtype=cache.dtype, device=cache.device)
     p.table, p.lengths, p.k_out, p.v_out = table.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr()
     L.check(ops._call(L.load().ha_paged_gather, cache.device, C.byref(p)), 'ha_paged_gather')
     return k, v

@@ -57,18 +57,18 @@ def test_entry_points_refuse_their_own(lib):
         assert lib.ha_paged_append(C.byref(_params(**over)), None) == -1, over
     for over in (dict(q=None), dict(o=None), dict(lse=None), dict(q=264), dict(q_sh=100), dict(H=0)):
         assert lib.ha_paged_attn(C.byref(_params(**over)), None) == -1, over
-    assert lib.ha_paged_attn(C.byref(_params()), None) == -3                                    # workspace too small
-    assert lib.ha_paged_attn(C.byref(_params(workspace=None)), None) == -3
+    assert lib.ha_paged_attn(C.byref(_params(columns=4000)), None) == -3                        # workspace too small
+    assert lib.ha_paged_attn(C.byref(_params(workspace=None, columns=4000)), None) == -3
     for over in (dict(rows=-1), dict(k_out=None), dict(v_out=264)):
         assert lib.ha_paged_gather(C.byref(_params(**over)), None) == -1, over
     for fn in (lib.ha_paged_append, lib.ha_paged_attn, lib.ha_paged_gather):
         assert fn(None, None) == -1
         assert fn(C.byref(_params(B=0)), None) == 0                                             # nothing to do
     assert lib.ha_launch_count() == launches
-    # workspace: two parts of 16 rows a CTA; never for more CTAs than there can be tiles
-    one = lib.ha_paged_attn_workspace_bytes(C.byref(_params(B=1, Hk=1, columns=1)))
-    assert one == 256 + 16 + 2 * 16 * (128 * 4 + 8)
-    assert lib.ha_paged_attn_workspace_bytes(C.byref(_params(B=0))) == 0
+    # workspace: two parts of 16 rows a CTA; none where a cluster shares an item
+    one = lib.ha_paged_attn_workspace_bytes(C.byref(_params(B=1, Hk=1, columns=4000)))
+    assert one == 256 + 296 * (16 + 2 * 16 * (128 * 4 + 8))
+    assert lib.ha_paged_attn_workspace_bytes(C.byref(_params(B=0))) == 0 and lib.ha_paged_attn_workspace_bytes(C.byref(_params())) == 0
     assert lib.ha_paged_attn_workspace_bytes(C.byref(_params(d=96))) == -1
 
 
