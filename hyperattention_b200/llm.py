@@ -9,6 +9,8 @@ the ChatGLM2-6B shape to run it in (benchmark configuration 4).
   13696, vocabulary 65024, 28 blocks), with the module nesting the patch expects
   (``model.transformer.encoder.layers[i].self_attention.core_attention``).  Weights are random (N(0, 0.02)); there
   is no checkpoint or tokenizer in this environment.  Everything outside the attention core is plain PyTorch.
+* ``DecoderCache`` and ``ChatGLM2ShapedDecoder.generate`` go on from a prompt token by token: keys and values, rotated, in a paged cache
+  of 16 or 4 bits (hyperattention_b200.paged), the new tokens' attention over its pages.
 """
 import math
 from types import SimpleNamespace
@@ -17,6 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from .module import HyperAttention
+from .paged import PagedCache, paged_append, paged_attn_func
 
 NUM_TOTAL_LAYERS = {
     'chatglm2-6b-32k': 28,
@@ -155,6 +158,39 @@ def _apply_rope(x, cache):
     return torch.cat([out.flatten(3), xp], dim=-1)
 
 
+class DecoderCache:
+    """Keys and values of every block for ``batch`` sequences of at most ``max_len`` tokens (rounded up to whole pages).
+
+    ``held`` int32 [batch]: tokens of each sequence in the cache; ``length``: an upper bound of them that the host knows.  ``rope``: cosines and sines by
+    position, fp32 (angles in 64 bits).  Sequence b has pages b * columns .. of the pool in order; any table of another kind will do as well."""
+
+    def __init__(self, config, batch, max_len, page_size=64, bits=16, dtype=torch.bfloat16, device='cuda'):
+        assert batch >= 1 and max_len >= 1 and page_size >= 1
+        self.columns = -(-max_len // page_size)
+        self.capacity = self.columns * page_size
+        self.batch, self.length = batch, 0
+        self.layers = [PagedCache.allocate(batch * self.columns, page_size, config.multi_query_group_num, config.kv_channels, dtype, bits, device)
+                       for _ in range(config.num_layers)]
+        self.table = torch.arange(batch * self.columns, dtype=torch.int32, device=device).view(batch, self.columns)
+        self.held = torch.zeros(batch, dtype=torch.int32, device=device)
+        rot = config.kv_channels // 2
+        inv = (10000.0 * config.rope_ratio) ** -(torch.arange(0, rot, 2, device=device, dtype=torch.float64) / rot)
+        ang = torch.outer(torch.arange(self.capacity, device=device, dtype=torch.float64), inv)
+        self.rope = torch.stack([ang.cos(), ang.sin()], -1).float()
+
+    def clear(self):
+        self.length = 0
+        self.held.zero_()
+
+
+class _Step:
+    """What the blocks of one cached forward share."""
+
+    def __init__(self, cache, n, counts, prompt):
+        self.cache, self.counts, self.prompt = cache, counts, prompt
+        self.total = cache.held + (n if counts is None else counts)
+
+
 class SelfAttention(torch.nn.Module):
     def __init__(self, config, layer_number):
         super().__init__()
@@ -164,14 +200,24 @@ class SelfAttention(torch.nn.Module):
         self.core_attention = ExactCoreAttention(config, layer_number)
         self.dense = torch.nn.Linear(proj, config.hidden_size, bias=False)
 
-    def forward(self, x, rope):
+    def forward(self, x, rope, step=None, layer=0):
         sq, b, _ = x.shape
         qkv = self.query_key_value(x)
         q, k, v = qkv.split([self.heads * self.hn, self.groups * self.hn, self.groups * self.hn], dim=-1)
         q = q.view(sq, b, self.heads, self.hn)
         k = k.view(sq, b, self.groups, self.hn)
         v = v.view(sq, b, self.groups, self.hn)
-        q, k = _apply_rope(q, rope), _apply_rope(k, rope)
+        if step is None:
+            q, k = _apply_rope(q, rope), _apply_rope(k, rope)
+        else:
+            cache, at = step.cache.layers[layer], step.cache
+            q, k, v = [t.transpose(0, 1) for t in (q, k, v)]                     # [b, sq, heads, hn], as the cache's operators take them
+            if not step.prompt:
+                q = paged_append(cache, k, v, at.table, at.held, step.counts, at.rope, q)
+                o, _ = paged_attn_func(q, cache, at.table, step.total, step.counts)
+                return self.dense(o.transpose(0, 1).reshape(sq, b, -1))
+            q, k = paged_append(cache, k, v, at.table, at.held, step.counts, at.rope, q, return_keys=True)
+            q, k, v = [t.transpose(0, 1) for t in (q, k, v)]
         rep = self.heads // self.groups
         # multi-query: every key/value group serves heads/groups query heads; expanded before the core, as the
         # attention core of the original model expects equal head counts
@@ -200,8 +246,8 @@ class GLMBlock(torch.nn.Module):
         self.post_attention_layernorm = RMSNorm(config.hidden_size, config.layernorm_epsilon)
         self.mlp = MLP(config)
 
-    def forward(self, x, rope):
-        x = x + self.self_attention(self.input_layernorm(x), rope)
+    def forward(self, x, rope, step=None, layer=0):
+        x = x + self.self_attention(self.input_layernorm(x), rope, step, layer)
         return x + self.mlp(self.post_attention_layernorm(x))
 
 
@@ -240,13 +286,59 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
                 elif name.endswith('bias'):
                     prm.zero_()
 
-    def forward(self, input_ids):
+    def forward(self, input_ids, cache=None, counts=None):
+        """Logits of a prompt.  With a DecoderCache, the tokens go on from what it holds, and are in it afterwards: into an empty cache a prompt of any length
+        (its attention is the blocks' own), behind that a few tokens a sequence (theirs goes over the pages).  counts: int32 [b], tokens of each
+        sequence where input_ids are padded on the right; logits of the padding mean nothing."""
         b, sq = input_ids.shape
+        if cache is None:
+            return self._run(input_ids, None)
+        assert b == cache.batch and len(cache.layers) == self.config.num_layers, 'the cache is for another batch or model'
+        assert cache.length + sq <= cache.capacity, f'the cache holds {cache.capacity} tokens a sequence'
+        prompt = cache.length == 0
+        cache.length += sq
+        return self._run(input_ids, _Step(cache, sq, counts, prompt))
+
+    def _run(self, input_ids, step):
+        sq = input_ids.shape[1]
         x = self.transformer.embedding(input_ids).transpose(0, 1).contiguous()      # [sq, b, hidden]
-        rope = _rope_cache(sq, self.config.kv_channels // 2, self.config.rope_ratio, x.device, x.dtype)
-        for layer in self.transformer.encoder.layers:
-            x = layer(x, rope)
+        rope = None if step is not None else _rope_cache(sq, self.config.kv_channels // 2, self.config.rope_ratio, x.device, x.dtype)
+        for i, layer in enumerate(self.transformer.encoder.layers):
+            x = layer(x, rope, step, i)
+        if step is not None:
+            step.cache.held.copy_(step.total)
         x = self.transformer.encoder.final_layernorm(x)
-        if self.last_only:
+        if self.last_only and (step is None or step.counts is None):
             x = x[-1:]
         return self.transformer.output_layer(x).transpose(0, 1)
+
+    @torch.no_grad()
+    def generate(self, input_ids, new_tokens, counts=None, cache=None, page_size=64, bits=16, graph=True):
+        """The most probable new_tokens tokens behind a prompt, one by one: int64 [b, new_tokens].  counts: int32 [b] prompt lengths where input_ids are padded
+        on the right.  cache: an empty DecoderCache to use; made for the call otherwise.  graph: the steps behind the second token replay a CUDA graph."""
+        b, sq = input_ids.shape
+        w = self.transformer.output_layer.weight
+        if cache is None:
+            cache = DecoderCache(self.config, b, sq + new_tokens, page_size, bits, w.dtype, w.device)
+        assert cache.length == 0, 'the cache is not empty'
+        out = torch.empty(b, new_tokens, dtype=torch.int64, device=input_ids.device)
+        if new_tokens == 0:
+            return out
+        logits = self(input_ids, cache, counts)
+        last = logits[:, -1] if counts is None else logits[torch.arange(b, device=logits.device), counts.long() - 1]
+        ids = last.argmax(-1, keepdim=True)
+        out[:, :1] = ids
+        replay = None
+        for i in range(1, new_tokens):
+            if replay is not None:
+                cache.length += 1
+                replay.replay()
+            else:
+                ids.copy_(self(ids, cache)[:, -1].argmax(-1, keepdim=True))
+                if graph and i + 2 < new_tokens:
+                    torch.cuda.current_stream().synchronize()
+                    replay = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(replay):
+                        ids.copy_(self._run(ids, _Step(cache, 1, None, False))[:, -1].argmax(-1, keepdim=True))
+            out[:, i:i + 1] = ids
+        return out

@@ -2,14 +2,16 @@
 attention of the last 14 of 28 blocks replaced by HyperAttention; reports prefill tokens/s of the all-exact and the
 patched model and the deviation of the last-position logits.
 
-    python -m hyperattention_b200.llm_bench [--seq-len 32768] [--layers 28] [--patch-layers 14] [--steps 3]
+    python -m hyperattention_b200.llm_bench [--seq-len 32768] [--layers 28] [--patch-layers 14] [--steps 3] [--new-tokens 0]
+
+--new-tokens N: also goes on from the prompt for N tokens, with a cache in 16 and in 4 bits, and reports the time of a token.
 """
 import argparse
 import json
 
 import torch
 
-from .llm import ChatGLM2ShapedDecoder, chatglm2_config, patch_attention_layers
+from .llm import ChatGLM2ShapedDecoder, DecoderCache, chatglm2_config, patch_attention_layers
 
 
 def main():
@@ -21,6 +23,7 @@ def main():
     ap.add_argument('--hidden', type=int, default=4096)
     ap.add_argument('--ffn', type=int, default=13696)
     ap.add_argument('--vocab', type=int, default=65024)
+    ap.add_argument('--new-tokens', type=int, default=0)
     a = ap.parse_args()
     assert torch.cuda.is_available()
     dev = torch.device('cuda')
@@ -50,6 +53,23 @@ def main():
         if hasattr(layer.self_attention.core_attention, 'grouped_kv'):
             layer.self_attention.core_attention.grouped_kv = True
     ms_grouped, logits_grouped = timed(lambda: model(ids))
+    def token_ms(bits):
+        """Time of one token behind the prompt: generation of N tokens less that of one, both with the prompt."""
+        cache = DecoderCache(cfg, 1, a.seq_len + a.new_tokens + 4, bits=bits)
+        times = []
+        for n in (4, a.new_tokens + 4):
+            cache.clear()
+            model.generate(ids, n, cache=cache)
+            cache.clear()
+            e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            e0.record()
+            model.generate(ids, n, cache=cache)
+            e1.record()
+            e1.synchronize()
+            times.append(e0.elapsed_time(e1))
+        return (times[1] - times[0]) / a.new_tokens
+
+    extra = {} if a.new_tokens <= 0 else {'new_tokens': a.new_tokens, 'ms_per_new_token_cache_16bit': token_ms(16), 'ms_per_new_token_cache_4bit': token_ms(4)}
     le, lh = logits_exact.float(), logits_hyper.float()
     dev_rel = ((lh - le).norm() / le.norm()).item()
     top1 = bool((le.argmax(-1) == lh.argmax(-1)).all())
@@ -58,7 +78,7 @@ def main():
                       'exact_tokens_per_s': a.seq_len / ms_exact * 1e3, 'hyper_tokens_per_s': a.seq_len / ms_hyper * 1e3,
                       'speedup': ms_exact / ms_hyper, 'last_logits_rel_deviation': dev_rel, 'last_token_top1_same': top1,
                       'hyper_grouped_kv_prefill_ms': ms_grouped, 'speedup_grouped_kv': ms_exact / ms_grouped,
-                      'grouped_vs_expanded_logits_rel_deviation': ((logits_grouped.float() - lh).norm() / lh.norm()).item()}))
+                      'grouped_vs_expanded_logits_rel_deviation': ((logits_grouped.float() - lh).norm() / lh.norm()).item(), **extra}))
 
 
 if __name__ == '__main__':
