@@ -1,4 +1,4 @@
-"""Builds libhyperattn_b200.so for sm_100a with nvcc, in-tree (next to the Python package).
+"""Builds libhyperattn_b200.so for sm_100a with nvcc, and the extension module _paged_ext.so with g++, in-tree (next to the Python package).
 
     python hyperattention_b200/csrc/build.py [--force] [--verbose] [--timing]
 
@@ -8,6 +8,7 @@ library, libhyperattn_b200_timing.so, with the kernels' per-phase cycle counters
 """
 import argparse
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -17,6 +18,7 @@ PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 SOURCES = ['stream_kernels.cu', 'seg_sort.cu', 'attn_simt.cu', 'attn_f32_tiled.cu', 'tensor_map.cu', 'attn_tc_fwd.cu', 'attn_tc_bwd.cu', 'attn_tc_bwd_ws.cu', 'attn_tc_bwd_kt.cu', 'attn_api.cu', 'causal.cu', 'paged_cache.cu', 'paged_attn.cu']
 LIB = os.path.join(PKG, 'libhyperattn_b200.so')
+EXT = os.path.join(PKG, '_paged_ext.so')
 NVCC_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-O3', '-std=c++17', '-lineinfo', '-Xcompiler', '-fPIC',
               '-I' + os.path.join(ROOT, 'include'), '-I' + HERE]
 
@@ -26,6 +28,28 @@ def _newer(path, deps):
         return True
     t = os.path.getmtime(path)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def build_ext(force=False, verbose=False):
+    """The Python operators of the paged cache (paged_ext.cpp) as an extension module, next to the library whose functions it is handed."""
+    src, header = os.path.join(HERE, 'paged_ext.cpp'), os.path.join(ROOT, 'include', 'hyperattn_b200.h')
+    if not force and not _newer(EXT, [src, header]):
+        return EXT
+    import sysconfig
+    import torch
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(os.environ.get('NVCC', 'nvcc')) or '/usr/local/cuda/bin/nvcc')))
+    include = [os.path.join(base, 'include'), os.path.join(base, 'include', 'torch', 'csrc', 'api', 'include'), sysconfig.get_paths()['include'],
+               os.path.join(cuda, 'include')]
+    cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC', '-I' + os.path.join(ROOT, 'include')] + ['-isystem' + i for i in include] + \
+        [f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', src, '-o', EXT, '-L' + os.path.join(base, 'lib'),
+         '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lc10', '-lc10_cuda']
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(' '.join(cmd) + '\n' + r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError('g++ failed for ' + src)
+    return EXT
 
 
 def build(force=False, verbose=False, timing=False):
@@ -65,6 +89,8 @@ def build(force=False, verbose=False, timing=False):
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError('link failed')
+    if not timing:
+        build_ext(force, verbose)
     return lib
 
 

@@ -15,14 +15,30 @@ neither written nor read and is reported by the next call into the library (or `
 operators have no gradient.
 """
 import ctypes as C
+import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import ops
 
 GROUP = 64          # elements of a row that share a step and an offset in a 4-bit cache
 _ROWS = (torch.bfloat16, torch.float16)
+_EXT = None
+
+
+def _ext():
+    """The operators' host side (csrc/paged_ext.cpp: checks, allocations and the call into the library), loaded once."""
+    global _EXT
+    if _EXT is None:
+        if not os.path.exists(os.path.join(os.path.dirname(L.LIB_PATH), '_paged_ext.so')):
+            raise RuntimeError('_paged_ext.so is missing: build it with `python hyperattention_b200/csrc/build.py` (there is no fallback implementation)')
+        from . import _paged_ext
+        lib = L.load()
+        _paged_ext.init(*[C.cast(getattr(lib, 'ha_paged_' + f), C.c_void_p).value for f in ('append', 'attn', 'gather', 'maps', 'attn_workspace_bytes')])
+        _EXT = _paged_ext
+    return _EXT
 
 
 class PagedCache:
@@ -73,10 +89,18 @@ class PagedCache:
             p.scale_sp, p.scale_sh, p.scale_st = k_scales.stride()[:3]
         for name, t in zip(('k_pages', 'v_pages', 'k_scales', 'v_scales'), self._tensors):
             setattr(p, name, t.data_ptr())
-        self._raw = bytes(p)             # the parameters of a call that the cache decides
-        self._at = [t.data_ptr() for t in self._tensors]
-        self._maps = None                # what the attention kernel keeps about 16-bit pages
-        self._plans = {}                 # parameters of calls by their tensors' shapes and strides (bounded); no pointers but the cache's own
+        self._params = p                 # the parameters of a call that the cache decides
+        self._handle = None
+
+    def _open(self):
+        """What the operators' host side keeps of the cache: made at the first call."""
+        host_word = 0
+        if self.device.type == 'cuda':
+            ops._status_words(self.device)
+            self._params.status, self._params.status_host = ops._STATUS_RAW[self.device.index][:2]
+            host_word = self._params.status_host
+        self._handle = _ext().open(bytes(self._params), host_word, *self._tensors)
+        return self._handle
 
     k = property(lambda self: self._tensors[0])
     v = property(lambda self: self._tensors[1])
@@ -104,59 +128,18 @@ class PagedCache:
             out.append((q * scales[..., :1].float() + scales[..., 1:].float()).flatten(-2))
         return tuple(out)
 
-    def _check_place(self):
-        assert [t.data_ptr() for t in self._tensors] == self._at, 'the pages have moved: make a new PagedCache'
 
-    def _plan(self, key, make):
-        """Parameters of a call whose tensors have the shapes, strides and types of `key`: checked and filled in once."""
-        plan = self._plans.get(key)
-        if plan is None:
-            p = L.PagedParams.from_buffer_copy(self._raw)
-            rest = make(p)
-            if len(self._plans) >= 256:
-                self._plans.clear()
-            plan = self._plans[key] = (bytes(p), rest)
-        return plan
-
-
-def _form(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
-
-
-# (an allocation of known strides costs a third less host time than torch.empty, and these calls are that time where the batch is small)
-_new = torch.empty_strided
-
-
-def _dense(*shape):
-    """Sizes and strides of a contiguous tensor."""
-    strides, n = [], 1
-    for s in reversed(shape):
-        strides.append(n)
-        n *= max(s, 1)
-    return shape, tuple(reversed(strides))
-
-
-def _places(p, cache, table, lengths, counts, B):
-    """Checks the table and the lengths of a call, and fills in their sizes."""
-    ops._cuda(cache.k)
-    dev = cache.device
-    assert table.dim() == 2 and table.shape[0] == B and table.dtype == torch.int32 and (table.stride(1) == 1 or table.shape[1] <= 1), \
-        'table must be int32 [batch, columns], rows contiguous'
-    assert lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.is_contiguous(), 'lengths must be contiguous int32 [batch]'
-    assert table.device == dev and lengths.device == dev, 'all tensors must be on one device'
-    if counts is not None:
-        assert counts.shape == (B,) and counts.dtype == torch.int32 and counts.is_contiguous() and counts.device == dev, \
-            'counts must be contiguous int32 [batch]'
-    p.B, p.columns, p.table_sb = B, table.shape[1], table.stride(0)
-
-
-def _rows(cache, t, B, n, heads, what):
-    assert t.dim() == 4 and t.shape == (B, n, heads, cache.head_dim), f'{what} must be [batch, tokens, heads, head_dim] with the head_dim of the cache'
-    assert t.dtype == cache.dtype and t.device == cache.device, f'{what} must have the type and device of the cache'
-
-
-def _no_grad(*ts):
-    assert not ops._wants_grad(*ts), 'the operators of the paged cache have no gradient: call them under torch.no_grad()'
+def _call(name, cache, *args):
+    # forward-mode differentiation and function transforms would lose their tangents without a word
+    assert forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active(), \
+        'the operators of the paged cache have no gradient: call them under torch.no_grad()'
+    r = getattr(_EXT or _ext(), name)(cache._handle or cache._open(), *args)
+    if r.__class__ is int:
+        L.check(r, 'ha_paged_' + name)
+    if r is NotImplemented:              # an earlier launch has reported a failure: raised here, as at every call into the library
+        ops._raise_if_failed(*ops._status_words(cache.device))
+        return _call(name, cache, *args)
+    return r
 
 
 def paged_append(cache, k, v, table, lengths, counts=None, rope=None, q=None, return_keys=False):
@@ -170,48 +153,7 @@ def paged_append(cache, k, v, table, lengths, counts=None, rope=None, q=None, re
 
     Returns the rotated queries [B, n, heads, head_dim] (None without q); with return_keys, (queries, rotated keys [B, n, kv_heads, head_dim]): what the
     prompt's own attention takes.  Padding rows of both are zero.  Two rows of one call must not go to the same slot."""
-    # rows that are not contiguous are copied, as in HyperAttention
-    k, v, q = [t if t is None or t.dim() == 0 or t.stride(-1) == 1 else t.contiguous() for t in (k, v, q)]
-    _no_grad(k, v) if q is None else _no_grad(k, v, q)
-
-    def make(p):
-        assert k.dim() == 4, 'k must be [batch, tokens, heads, head_dim]'
-        B, p.n = k.shape[:2]
-        _places(p, cache, table, lengths, counts, B)
-        _rows(cache, k, B, p.n, cache.kv_heads, 'k')
-        _rows(cache, v, B, p.n, cache.kv_heads, 'v')
-        p.k_sb, p.k_sn, p.k_sh, _ = k.stride()
-        p.v_sb, p.v_sn, p.v_sh, _ = v.stride()
-        if q is not None:
-            assert q.dim() == 4 and q.shape[2] % cache.kv_heads == 0, 'query heads must be a multiple of the key/value heads'
-            _rows(cache, q, B, p.n, q.shape[2], 'q')
-            p.H = q.shape[2]
-            p.q_sb, p.q_sn, p.q_sh, _ = q.stride()
-        if rope is not None:
-            assert rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous() and rope.device == cache.device, 'rope must be contiguous [positions, rot / 2, 2]'
-            assert rope.dtype in (torch.float32, cache.dtype) and 2 * rope.shape[1] <= cache.head_dim, \
-                'rope must be fp32 or of the cache\'s type, for at most head_dim elements'
-            p.rot, p.rope_rows, p.rope_dtype = 2 * rope.shape[1], rope.shape[0], ops._DT[rope.dtype]
-        return _dense(*k.shape), None if q is None else _dense(*q.shape)
-
-    cache._check_place()
-    raw, (k_form, q_form) = cache._plan(('append', _form(k), _form(v), _form(q), _form(table), _form(lengths), _form(counts), _form(rope)), make)
-    p = L.PagedParams.from_buffer_copy(raw)
-    ops._set_status(p, cache.device)
-    p.k, p.v, p.table, p.lengths = k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr()
-    q_out = k_out = None
-    if counts is not None:
-        p.counts = counts.data_ptr()
-    if rope is not None:
-        p.rope = rope.data_ptr()
-    if q is not None:
-        q_out = _new(*q_form, dtype=cache.dtype, device=cache.device)
-        p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
-    if return_keys:
-        k_out = _new(*k_form, dtype=cache.dtype, device=cache.device)
-        p.k_out = k_out.data_ptr()
-    L.check(ops._call(L.load().ha_paged_append, cache.device, C.byref(p)), 'ha_paged_append')
-    return (q_out, k_out) if return_keys else q_out
+    return _call('append', cache, k, v, table, lengths, counts, rope, q, return_keys)
 
 
 def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
@@ -223,63 +165,10 @@ def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
     Row i < counts[b] sees positions 0 .. lengths[b] - counts[b] + i.  A row that sees none, and padding rows, have o = 0 and lse = -inf.  Consecutive
     query heads share a K/V head.  Every token reads the sequence's keys again (from the L2 cache where they fit): made for one to a few
     tokens a sequence; prompts belong to HyperAttention or flash_attn_func."""
-    _no_grad(q)
-    if q.dim() == 4 and (q.stride(3) != 1 or (q.data_ptr() | 2 * (q.stride(0) | q.stride(1) | q.stride(2))) % 16):
-        q = q.clone(memory_format=torch.contiguous_format)             # rows that the kernel's 16-byte loads cannot read
-    scale = float(softmax_scale or cache.head_dim ** -0.5)
-
-    def make(p):
-        assert q.dim() == 4 and q.shape[2] % cache.kv_heads == 0 and q.shape[2] > 0, 'q must be [batch, tokens, heads, head_dim], heads a multiple of the K/V heads'
-        B, p.n, p.H, _ = q.shape
-        _rows(cache, q, B, p.n, p.H, 'q')
-        _places(p, cache, table, lengths, counts, B)
-        p.q_sb, p.q_sn, p.q_sh, _ = q.stride()
-        p.scale = scale
-        lib = L.load()
-        with torch.cuda.device(cache.device):
-            if cache.bits == 16 and cache._maps is None:
-                maps = C.create_string_buffer(256)
-                L.check(lib.ha_paged_maps(C.byref(p), maps), 'ha_paged_maps')
-                cache._maps = maps
-            p.maps = None if cache._maps is None else C.addressof(cache._maps)
-            nbytes = lib.ha_paged_attn_workspace_bytes(C.byref(p))
-        L.check(min(nbytes, 0), 'ha_paged_attn')
-        return nbytes, _dense(*q.shape), _dense(B, p.H, p.n)
-
-    cache._check_place()
-    raw, (nbytes, form, lse_form) = cache._plan(('attn', _form(q), _form(table), _form(lengths), _form(counts), scale), make)
-    dev = cache.device
-    o = _new(*form, dtype=cache.dtype, device=dev)
-    lse = _new(*lse_form, dtype=torch.float32, device=dev)
-    p = L.PagedParams.from_buffer_copy(raw)
-    ops._set_status(p, dev)
-    p.q, p.table, p.lengths, p.o, p.lse = q.data_ptr(), table.data_ptr(), lengths.data_ptr(), o.data_ptr(), lse.data_ptr()
-    if nbytes:
-        ws = _new((nbytes,), (1,), dtype=torch.uint8, device=dev)        # (free once the launches are enqueued: same stream)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
-    if counts is not None:
-        p.counts = counts.data_ptr()
-    L.check(ops._call(L.load().ha_paged_attn, dev, C.byref(p)), 'ha_paged_attn')
-    return o, lse
+    return _call('attn', cache, q, table, lengths, counts, float(softmax_scale or cache.head_dim ** -0.5))
 
 
 def paged_gather(cache, table, lengths, rows):
     """Positions 0 .. rows - 1 of every sequence as dense (k, v) [B, kv_heads, rows, head_dim] in the cache's type, zero from lengths[b] (int32 [B]) on: the
     layout that HyperAttention takes."""
-    rows = int(rows)
-
-    def make(p):
-        assert table.dim() == 2 and rows >= 0, 'table must be int32 [batch, columns], rows a number'
-        _places(p, cache, table, lengths, None, table.shape[0])
-        p.rows = rows
-        return _dense(table.shape[0], cache.kv_heads, rows, cache.head_dim)
-
-    cache._check_place()
-    raw, form = cache._plan(('gather', _form(table), _form(lengths), rows), make)
-    p = L.PagedParams.from_buffer_copy(raw)
-    ops._set_status(p, cache.device)
-    k = _new(*form, dtype=cache.dtype, device=cache.device)
-    v = _new(*form, dtype=cache.dtype, device=cache.device)
-    p.table, p.lengths, p.k_out, p.v_out = table.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr()
-    L.check(ops._call(L.load().ha_paged_gather, cache.device, C.byref(p)), 'ha_paged_gather')
-    return k, v
+    return _call('gather', cache, table, lengths, int(rows))
