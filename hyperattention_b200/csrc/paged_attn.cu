@@ -2,9 +2,9 @@
 //
 //   s_j = scale q . k_j,  o = sum_j exp(s_j) v_j / sum_j exp(s_j),  lse = log sum_j exp(s_j),  j < keys of the row
 //
-// An item is the (up to 16) query heads of one token that share a K/V head: the 16 rows of mma.sync.m16n8k16, which is what one pass over the
-// keys can serve.  The products are thin (16 query rows against all keys), and K and V are read once: bytes bound the kernel.
-// A query row sees all or none of an item's keys, so that no masked value meets a product with weight 0.
+// An item is the query rows that share a K/V head, up to 16, the rows of mma.sync.m16n8k16: the heads of one token, or of a few neighbouring tokens
+// where they are less than that.  The products are thin (16 query rows against all keys), and K and V are read once: bytes bound the kernel.
+// Tokens of an item see the same keys but for the last few; a value there that is no number is kept from the rows that do not see it.
 //
 // All items' keys, in tiles of TK, form one list; CTA c takes the c-th equal part of it, whatever the lengths are.  An item that lies within one CTA is
 // finished there; of one that crosses to the next, each CTA writes its part (unnormalised sums, reference, denominator) to the workspace,
@@ -36,7 +36,7 @@ struct Stage {
   static constexpr int V = TK * ROW, Q = 2 * TK * ROW, BYTES = Q + ITEM_ROWS * ROW;
   static constexpr int CTAS = D == 128 ? 2 : 3, NS = D == 128 ? 3 : 4;
   static constexpr int BARS = 2 * NS + 1;
-  static constexpr int SMEM = NS * BYTES + 4 * ITEM_ROWS * 8 + BARS * 8 + (2 * MAX_LINES + 8) * 4 + 16;
+  static constexpr int SMEM = NS * BYTES + 4 * ITEM_ROWS * 8 + BARS * 8 + (2 * MAX_LINES + 8) * 4 + 16 + MAX_LINES;
   static_assert(4 * ITEM_ROWS * D * 4 <= Q, "the warps' sums fit a stage");
   static_assert(ITEM_ROWS * (D * 4 + 8) <= BYTES, "... and a cluster's part");
   static_assert(BYTES % 1024 == 0, "stages begin on the swizzle's boundary");
@@ -48,7 +48,7 @@ struct Stage {
 template <int TK>
 __device__ __forceinline__ uint32_t slab_at(int row, int chunk) { return (chunk >> 3) * (TK * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 
-template <typename T, int D>
+template <typename T, int D, bool PACKED>
 struct Worker {
   using S = Stage<D>;
   static constexpr int ROWS = 16, ROUNDS = 1;
@@ -108,8 +108,47 @@ struct Worker {
     __syncwarp();
   }
 
-  // One tile: this warp's keys, of which the first `left` exist.
-  __device__ __forceinline__ void tile(const uint8_t* stage, int left, float scale_log2) {
+  // Where the tokens of a pack see different keys: is there a value among this warp's rows of V that is no number?  Weight 0 would not take it out.
+  __device__ __forceinline__ bool infinite(const uint8_t* stage) const {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr uint32_t EXP = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    bool found = false;
+    for (int e = lane; e < S::KW * (D / 8); e += 32) {
+      const uint4 v = lds128(stage + S::V + slab_at<S::TK>(warp * S::KW + e / (D / 8), e % (D / 8)));
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int y = 0; y < 4; ++y) found = found || (w[y] & EXP) == EXP || ((w[y] >> 16) & EXP) == EXP;
+    }
+    return __any_sync(0xffffffffu, found);
+  }
+  // ... then each row takes the values of the keys that it sees, one by one.
+  __device__ __forceinline__ void add_singly(const AttnArgs& a, const uint8_t* stage, int left, int last, const float (&p)[NT][4]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
+    const int sees[2] = {left - keys_short<PACKED>(a, lane >> 2, last), left - keys_short<PACKED>(a, (lane >> 2) + 8, last)};
+#pragma unroll 1
+    for (int key = 0; key < S::KW; ++key) {
+      float w[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float even = key < 8 ? p[0][2 * r] : p[1][2 * r], odd = key < 8 ? p[0][2 * r + 1] : p[1][2 * r + 1];
+        w[r] = __shfl_sync(0xffffffffu, key & 1 ? odd : even, (lane & ~3) | ((key & 7) >> 1));
+      }
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        const float2 v = unpack2<T>(lds32(stage + S::V + slab_at<S::TK>(warp * S::KW + key, j) + 4 * c));
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (key < sees[r]) {
+            acc[j][2 * r] = fmaf(w[r], v.x, acc[j][2 * r]);
+            acc[j][2 * r + 1] = fmaf(w[r], v.y, acc[j][2 * r + 1]);
+          }
+      }
+    }
+  }
+
+  // One tile: this warp's keys, of which the line's last token, the `last`-th of its pack, sees the first `left`.
+  __device__ __forceinline__ void tile(const AttnArgs& a, const uint8_t* stage, int left, int last) {
+    const float scale_log2 = a.scale_log2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
     const uint32_t at = smem_u32(stage);
     float x[NT][4];
@@ -125,12 +164,13 @@ struct Worker {
       mma16816<T>(x[0], qf[ks], b[0], b[1]);
       mma16816<T>(x[1], qf[ks], b[2], b[3]);
     }
-    if (left < S::KW) {
+    if (left - last < S::KW) {
+      const int sees[2] = {left - keys_short<PACKED>(a, lane >> 2, last), left - keys_short<PACKED>(a, (lane >> 2) + 8, last)};
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (t * 8 + 2 * c + (e & 1) >= left) x[t][e] = -INFINITY;
+          if (t * 8 + 2 * c + (e & 1) >= sees[e >> 1]) x[t][e] = -INFINITY;
     }
     const float top[2] = {fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]))};
     if (__any_sync(0xffffffffu, top[0] > limit[0] || top[1] > limit[1])) raise(top, scale_log2);
@@ -143,8 +183,8 @@ struct Worker {
       for (int r = 0; r < 2; ++r) {
         float p0, p1;
         unpack_f2(ffma2(pack_f2(x[t][2 * r], x[t][2 * r + 1]), dup_f2(scale_log2), dup_f2(-shift[r])), p0, p1);
-        p0 = fast_exp2(p0);
-        p1 = fast_exp2(p1);
+        x[t][2 * r] = p0 = fast_exp2(p0);
+        x[t][2 * r + 1] = p1 = fast_exp2(p1);
         sum[r] = fadd2(sum[r], pack_f2(p0, p1));
         const uint32_t w = pack2<T>(p0, p1);
         const float2 f = unpack2<T>(w);
@@ -152,6 +192,10 @@ struct Worker {
         lo[2 * t + r] = pack2<T>(p0 - f.x, p1 - f.y);
       }
     const int vrow = warp * S::KW + (lane & 15);
+    if (PACKED && last > 0 && left > 0 && left - last < S::KW && infinite(stage)) {
+      add_singly(a, stage, left, last, x);
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       uint32_t b[4];
@@ -200,7 +244,7 @@ __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap
     slot = 0;
     const int key = w.tile * TK + (r << a.run_log2);
     if (w.line >= lines || (r << a.run_log2) >= TK || key >= keys[w.line]) return 0;
-    return paged_entry(a.c, a.by_n(line0 + w.line), key, slot);
+    return paged_entry(a.c, a.by_packs(line0 + w.line), key, slot);
   };
   int slot, page = look_up(at, lane, slot);
   int s = 0;
@@ -213,7 +257,6 @@ __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap
     if (it + 1 == end) next.line = lines;
     int next_slot;
     const int next_page = look_up(next, lane, next_slot);              // (under way while this tile's copies are started)
-    const int b = a.by_n(line0 + at.line), i = line0 + at.line - b * a.n;
     const int h = a.by_blocks(at.item), left = keys[at.line] - at.tile * TK;
     for (int r0 = 0; (r0 << a.run_log2) < min(TK, left); r0 += 32) {
       if (r0 > 0) page = look_up(at, r0 + lane, slot);                 // (runs of less than TK / 32 rows)
@@ -227,13 +270,13 @@ __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap
       }
     }
     if (it == begin || at.tile == 0) {
-      const int block = at.item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
-      const uint8_t* q = a.q + b * a.q_sb + i * a.q_sn + (int64_t)(h * a.group + block * ITEM_ROWS) * a.q_sh;
+      const uint8_t* q = query_of(a, line0 + at.line, at.item);
       constexpr int C = 2 * D / 16;
 #pragma unroll
       for (int e = lane; e < ITEM_ROWS * C; e += 32) {
         const int r = e / C, chunk = e % C;
-        cp_async16(dst + S::Q + r * 2 * D + chunk_at(r, chunk) * 16, q + (r < rows ? r : 0) * a.q_sh + chunk * 16, r < rows ? 16 : 0);
+        const bool there = row_at(a, line0 + at.line, at.item, r).there;
+        cp_async16(dst + S::Q + r * 2 * D + chunk_at(r, chunk) * 16, q + (there ? query_row(a, r) : 0) + chunk * 16, there ? 16 : 0);
       }
     }
     cp_async_arrive(full);
@@ -253,7 +296,7 @@ __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap
   }
 }
 
-template <typename T, int D, bool CLUSTER>
+template <typename T, int D, bool CLUSTER, bool PACKED>
 __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     paged_attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm) {
   using S = Stage<D>;
@@ -265,6 +308,7 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
   int* keys = first + MAX_LINES + 4;                                         // [lines]
   const uint32_t base = smem_u32(smem), bars = smem_u32(keys + MAX_LINES);   // full[NS], empty[NS], join
   int* warp_sum = keys + MAX_LINES + 2 * S::BARS;                            // [4]
+  uint8_t* lasts = reinterpret_cast<uint8_t*>(warp_sum + 4);                 // [lines]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int items = a.Hk * a.blocks;
   if (tid == 0) {
@@ -281,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
   if (CLUSTER) chain_release();              // (short kernels, fewer CTAs than there is room for: the next one may be placed at once)
   chain_wait();
   int begin, end, line0;
-  Walk at = take_part<T, D, CLUSTER>(a, TK, first, keys, warp_sum, items, begin, end, line0);
+  Walk at = take_part<T, D, CLUSTER>(a, TK, first, keys, lasts, warp_sum, items, begin, end, line0);
   const int lines = CLUSTER ? 1 : a.lines, item = at.item;
   if (begin >= end && (!CLUSTER || keys[0] == 0)) return;
   if (warp == 4) {
@@ -294,7 +338,7 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     return;
   }
 
-  Worker<T, D> w;
+  Worker<T, D, PACKED> w;
   const uint32_t join_bar = bars + 8 * 2 * NS;
   uint32_t joined = 0;
   auto join = [&]() {
@@ -316,10 +360,12 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     if (it == begin || at.tile == 0) w.begin(stage, a);
     const int left = keys[at.line] - at.tile * TK - warp * S::KW;
     if (left < S::KW) w.clear_tail(stage, left);
-    w.tile(stage, left, a.scale_log2);
+    const int last = PACKED ? lasts[at.line] : 0;
+    w.tile(a, stage, left, last);
     const bool ends = at.tile == at.tiles - 1 || it == end - 1;
     if (ends) {
-      ok = finish_item<T, D, 16 * D, CLUSTER>(a, w, stat, reinterpret_cast<float*>(stage), at, first, items, begin, end, it == end - 1, line0, cluster_sums, cluster_stat, join);
+      ok = finish_item<T, D, 16 * D, CLUSTER>(a, w, stat, reinterpret_cast<float*>(stage), at, first, items, begin, end, it == end - 1, line0, keys[at.line], last, cluster_sums, cluster_stat,
+                                              join);
       if (!ok) break;
     }
     // the stage is free (what was written to it by stores before what copies write to it next)
@@ -331,10 +377,10 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
   }
   if constexpr (CLUSTER) {
     if (begin >= end || !ok) {
-      if (tid < ITEM_ROWS) cluster_stat[tid] = make_float2(-INFINITY, 0.f);
+      if (tid < ITEM_ROWS) cluster_stat[tid] = make_float2(-INFINITY, -1.f);
     }
     __syncwarp();
-    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, item);
+    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, item, keys[0], lasts[0]);
   }
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   chain_release();
@@ -351,8 +397,10 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const AttnArgs a) {
   if ((int64_t)(c + 1) * per >= total) return;
   const int4 hd = a.head[c];
   if (hd.y <= (c + 1) * per || hd.x < c * per) return;                 // ends here, or began before
-  const int h = a.by_blocks(hd.w), block = hd.w - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
-  if (row >= rows) return;
+  int token;
+  const int keys = keys_of(a, hd.z, token);
+  const RowAt ra = row_at(a, hd.z, hd.w, row, keys, token);
+  if (!ra.there) return;
   const int last = (hd.y - 1) / per, pieces = last - c + 1;
   auto slot = [&](int p) { return 2 * (c + p) + (p == 0 && hd.x > c * per ? 1 : 0); };
   float m = -INFINITY;
@@ -379,8 +427,8 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const AttnArgs a) {
       const float2 f = *reinterpret_cast<const float2*>(src);
       y[0] = f.x, y[1] = f.y;
     }
-    if (st.x != -INFINITY) {
-      const float w = fast_exp2(st.x - m);
+    {
+      const float w = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m);
       l = fmaf(w, st.y, l);
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = fmaf(w, y[e], v[e]);
@@ -391,21 +439,27 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const AttnArgs a) {
   if (lane == 0) red_l[warp] = l;
   __syncthreads();
   l = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
-  const int head = h * a.group + block * ITEM_ROWS + row;
-  const int b = a.by_n(hd.z), i = hd.z - b * a.n;
-  if (tid < D) ((T*)a.o)[((int64_t)hd.z * a.H + head) * D + tid] = from_f32<T>(((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) / l);
-  if (tid == 0) a.lse[((int64_t)b * a.H + head) * a.n + i] = (m + log2f(l)) * LN2;
+  if (tid < D) ((T*)a.o)[ra.o * D + tid] = from_f32<T>(ra.empty ? 0.f : ((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) / l);
+  if (tid == 0) a.lse[ra.lse] = ra.empty ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
 int attn_tile(const ha_paged_params& p) { return p.bits == 16 ? Stage<64>::TK : attn4_tile(p.d); }
+// Tokens of a sequence that share an item's rows, and items of a (pack, K/V head).
+int attn_pack(const ha_paged_params& p) {
+  const int group = p.H / p.Hk, most = group < ITEM_ROWS ? ITEM_ROWS / group : 1;
+  return p.n < most ? (p.n > 0 ? p.n : 1) : most;
+}
+int64_t attn_packs(const ha_paged_params& p) { return ((int64_t)p.n + attn_pack(p) - 1) / attn_pack(p); }
+int attn_rows(const ha_paged_params& p) { return p.H / p.Hk * attn_pack(p); }
+int attn_items(const ha_paged_params& p) { return p.Hk * ((p.H / p.Hk + ITEM_ROWS - 1) / ITEM_ROWS); }
 int attn_resident(const ha_paged_params& p) {
   if (p.bits == 16) return p.d == 128 ? Stage<128>::CTAS : Stage<64>::CTAS;
-  return attn4_resident(p.d, p.H / p.Hk);
+  return attn4_resident(p.d, attn_rows(p));
 }
 
 // CTAs of a launch over `lines` lines: as many as are resident at once, and no more than there can be tiles.
 int attn_ctas(const ha_paged_params& p, int lines) {
-  const int tk = attn_tile(p), items = p.Hk * ((p.H / p.Hk + ITEM_ROWS - 1) / ITEM_ROWS);
+  const int tk = attn_tile(p), items = attn_items(p);
   const int64_t most = ((int64_t)p.columns * p.page_size + tk - 1) / tk * items * lines;
   const int resident = sm_count() * attn_resident(p);
   return (int)(most < 1 ? 1 : most < resident ? most : resident);
@@ -415,7 +469,7 @@ int attn_ctas(const ha_paged_params& p, int lines) {
 // second launch (1 x 515 tokens: 8.1 -> 5.5 us on the device, 7 -> 4 us of host time).  Every item gets the same CTAs, however long it is, so that the list of tiles,
 // which deals them out evenly, is for what takes longer than the joining.
 int attn_cluster(const ha_paged_params& p) {
-  const int64_t units = (int64_t)p.B * p.n * p.Hk * ((p.H / p.Hk + ITEM_ROWS - 1) / ITEM_ROWS);
+  const int64_t units = p.B * attn_packs(p) * attn_items(p);
   const int64_t tiles = ((int64_t)p.columns * p.page_size + attn_tile(p) - 1) / attn_tile(p), resident = (int64_t)sm_count() * attn_resident(p);
   if (units > resident || tiles == 0) return 0;
   int c = 1;
@@ -425,8 +479,8 @@ int attn_cluster(const ha_paged_params& p) {
 
 // Lines of one launch: no more than shared memory counts, their tiles within 31 bits.
 int64_t attn_lines(const ha_paged_params& p) {
-  const int tk = attn_tile(p), items = p.Hk * ((p.H / p.Hk + ITEM_ROWS - 1) / ITEM_ROWS);
-  const int64_t tiles = ((int64_t)p.columns * p.page_size + tk - 1) / tk * items, all = (int64_t)p.B * p.n;
+  const int tk = attn_tile(p), items = attn_items(p);
+  const int64_t tiles = ((int64_t)p.columns * p.page_size + tk - 1) / tk * items, all = p.B * attn_packs(p);
   int64_t lines = all < MAX_LINES ? all : MAX_LINES;
   if (tiles > 0 && lines > (0x7fffffffLL - 65536) / tiles) lines = (0x7fffffffLL - 65536) / tiles;
   return lines;
@@ -449,13 +503,20 @@ int launch_attn(const AttnArgs& a, const ha_paged_params& p, int ctas, cudaStrea
   CUtensorMap maps[2] = {};
   if (p.maps) memcpy(maps, p.maps, sizeof(maps));
   else if (!attn_maps(p, maps)) return HA_ERR_INVALID;
-  if (a.cluster > 0) {
-    HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D, true>), S::SMEM, "ha_paged_attn");
-    launch_chained_clusters(paged_attn_kernel<T, D, true>, ctas, THREADS, S::SMEM, a.cluster, st, a, maps[0], maps[1]);
-  } else {
-    HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D, false>), S::SMEM, "ha_paged_attn");
-    launch_chained(paged_attn_kernel<T, D, false>, ctas, THREADS, S::SMEM, st, a, maps[0], maps[1]);
-  }
+  auto launch = [&](auto kernel) {
+    if (a.cluster > 0) launch_chained_clusters(kernel, ctas, THREADS, S::SMEM, a.cluster, st, a, maps[0], maps[1]);
+    else launch_chained(kernel, ctas, THREADS, S::SMEM, st, a, maps[0], maps[1]);
+  };
+#define HA_PAGED_VARIANT(cluster, packed)                                                          \
+  do {                                                                                             \
+    HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D, cluster, packed>), S::SMEM, "ha_paged_attn");       \
+    launch(paged_attn_kernel<T, D, cluster, packed>);                                              \
+  } while (0)
+  if (a.cluster > 0 && a.pack > 1) HA_PAGED_VARIANT(true, true);
+  else if (a.cluster > 0) HA_PAGED_VARIANT(true, false);
+  else if (a.pack > 1) HA_PAGED_VARIANT(false, true);
+  else HA_PAGED_VARIANT(false, false);
+#undef HA_PAGED_VARIANT
   HA_LAUNCHED("ha_paged_attn");
   return HA_OK;
 }
@@ -496,7 +557,7 @@ int64_t ha_paged_attn_workspace_bytes(const ha_paged_params* pp) {
   if ((p.bits != 16 && p.bits != 4) || (p.d != 64 && p.d != 128) || p.B < 0 || p.n < 0 || p.Hk < 1 || p.H < 1 || p.H % p.Hk != 0 || p.columns < 0 || p.page_size < 1)
     return HA_ERR_INVALID;
   if ((int64_t)p.columns * p.page_size > 0x7fffffffLL) return HA_ERR_TOO_LARGE;
-  const int64_t all = (int64_t)p.B * p.n, lines = attn_lines(p);
+  const int64_t all = p.B * attn_packs(p), lines = attn_lines(p);
   if (all == 0 || attn_cluster(p) > 0) return 0;
   return lines < 1 ? (int64_t)HA_ERR_TOO_LARGE : attn_workspace(p, attn_ctas(p, (int)lines));
 }
@@ -517,7 +578,8 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   a.q_sb = p.q_sb * 2; a.q_sn = p.q_sn * 2; a.q_sh = p.q_sh * 2;
   a.o = p.o; a.lse = p.lse;
   a.n = p.n; a.H = p.H; a.Hk = p.Hk; a.group = p.H / p.Hk; a.blocks = (a.group + ITEM_ROWS - 1) / ITEM_ROWS;
-  a.by_n = FastDiv((uint32_t)p.n); a.by_blocks = FastDiv((uint32_t)a.blocks);
+  a.pack = attn_pack(p); a.packs = (int)attn_packs(p);
+  a.by_packs = FastDiv((uint32_t)a.packs); a.by_blocks = FastDiv((uint32_t)a.blocks); a.by_group = FastDiv((uint32_t)a.group);
   a.scale_log2 = fabsf(p.scale) * LOG2E;
   a.flip = p.scale < 0.f ? 0x80008000u : 0u;
   a.cluster = cluster;
@@ -535,7 +597,7 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   }
   const cudaStream_t st = (cudaStream_t)stream;
   const bool bf = p.dtype == HA_BF16;
-  const int64_t all = (int64_t)p.B * p.n, most = cluster > 0 ? all : attn_lines(p);
+  const int64_t all = p.B * attn_packs(p), most = cluster > 0 ? all : attn_lines(p);
   for (int64_t line0 = 0; line0 < all; line0 += most) {
     a.line0 = (int)line0;
     a.lines = (int)(all - line0 < most ? all - line0 : most);
@@ -546,7 +608,7 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
     else rc = bf ? launch_attn<__nv_bfloat16, 128>(a, p, now, st) : launch_attn<__half, 128>(a, p, now, st);
     if (rc != HA_OK) return rc;
     if (now == 1 || cluster > 0) continue;
-    const dim3 grid(now - 1, a.group < ITEM_ROWS ? a.group : ITEM_ROWS);
+    const dim3 grid(now - 1, attn_rows(p) < ITEM_ROWS ? attn_rows(p) : ITEM_ROWS);
     if (p.d == 64) {
       if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 64>, grid, 128, 0, st, a);
       else launch_chained(paged_combine_kernel<__half, 64>, grid, 128, 0, st, a);

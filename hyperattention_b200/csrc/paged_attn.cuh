@@ -6,8 +6,8 @@
 namespace ha {
 
 constexpr int attn4_tile(int d) { return d == 128 ? 128 : 256; }      // keys of a tile of 4-bit rows
-constexpr int ITEM_ROWS = 16;         // query heads of an item, at most
-constexpr int MAX_LINES = 256;        // (sequence, token) pairs of one launch: their tiles are summed up in shared memory
+constexpr int ITEM_ROWS = 16;         // query rows of an item, at most
+constexpr int MAX_LINES = 256;        // lines (packs of a sequence's tokens) of one launch: their tiles are summed up in shared memory
 // A weight's reference follows the running maximum only when that is 2^SLACK above it: with 16 rows a warp, some row's maximum grows at most of the first
 // dozens of tiles, and each time all the sums are scaled.  Weights, held in 16 bits for the products, have that much room above.
 constexpr float SLACK = 6.f;
@@ -20,11 +20,12 @@ struct AttnArgs {
   void* o;
   float* lse;
   int32_t n, H, Hk, group, blocks;    // blocks: items of a (token, K/V head): group / 16, rounded up
-  int32_t line0, lines;               // (sequence, token) pairs of this launch
+  int32_t pack, packs;                // neighbouring tokens of a sequence that share an item (pack * group <= 16, or one), and how many packs a sequence has
+  int32_t line0, lines;               // (sequence, pack) pairs of this launch
   int32_t cluster;                    // CTAs that share an item, a cluster of them; 0: the list of tiles
   int32_t run_log2;                   // rows that are fetched together: 2^run_log2, the largest power of two that pages and tiles are made of
   int32_t whole_runs;                 // 4 bits: a warp's keys of a tile lie together, and their scales, on 16-byte boundaries
-  FastDiv by_n, by_blocks;
+  FastDiv by_packs, by_blocks, by_group;
   float scale_log2;                   // magnitude of the softmax scale, times log2 e
   uint32_t flip;                      // sign bits of a pair of queries, where the scale is negative
   float* part;                        // [CTAs][2][ITEM_ROWS][D], then ...
@@ -105,20 +106,50 @@ struct Walk {
 
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }      // 16-byte chunk of a query row in shared memory
 
-// Keys that a line (a token of a sequence) sees.
-__device__ __forceinline__ int keys_of(const AttnArgs& a, int line) {
-  const int b = a.by_n(line), i = line - b * a.n;
+// Keys that a line sees, those of its last token that is one of the sequence; `last`: that token's place in the pack.
+__device__ __forceinline__ int keys_of(const AttnArgs& a, int line, int& last) {
+  const int b = a.by_packs(line), i0 = (line - b * a.packs) * a.pack;
   const int count = a.c.counts ? min(a.c.counts[b], a.n) : a.n;
   int len = a.c.lengths[b];
   if (len > a.c.capacity) {
     report_status(a.c.status, a.c.status_host, HA_DEV_BAD_INDEX);
     len = a.c.capacity;
   }
-  return i < count ? max(max(len, 0) - (count - 1 - i), 0) : 0;
+  last = max(min(a.pack, count - i0) - 1, 0);
+  return i0 < count ? max(max(len, 0) - (count - 1 - i0 - last), 0) : 0;
+}
+// Keys that row `row` of an item does not see of those that the line's last token does: one for each token between (rows of padding like the last).
+template <bool PACKED>
+__device__ __forceinline__ int keys_short(const AttnArgs& a, int row, int last) { return PACKED ? max(last - a.by_group(row), 0) : 0; }
+
+// What row `row` of an item is.
+struct RowAt {
+  int64_t o, lse;                     // its outputs: a row of o, an element of lse
+  bool there, empty;                  // one of the call's rows; one of padding, or without keys
+};
+// (keys, last: what keys_of says of the line)
+__device__ __forceinline__ RowAt row_at(const AttnArgs& a, int line, int item, int row, int keys = 1, int last = 0) {
+  const int b = a.by_packs(line), i0 = (line - b * a.packs) * a.pack, h = a.by_blocks(item), block = item - h * a.blocks;
+  const int t = a.by_group(row), of_group = block * ITEM_ROWS + row - t * a.group, i = i0 + t, head = h * a.group + of_group;
+  RowAt r;
+  r.there = t < a.pack && i < a.n && of_group < a.group;
+  r.empty = t > last || keys <= last - t;
+  r.o = ((int64_t)b * a.n + i) * a.H + head;
+  r.lse = ((int64_t)b * a.H + head) * a.n + i;
+  return r;
+}
+// ... and its query, from the first row's on.
+__device__ __forceinline__ const uint8_t* query_of(const AttnArgs& a, int line, int item) {
+  const int b = a.by_packs(line), i0 = (line - b * a.packs) * a.pack, h = a.by_blocks(item), block = item - h * a.blocks;
+  return a.q + b * a.q_sb + i0 * a.q_sn + (int64_t)(h * a.group + block * ITEM_ROWS) * a.q_sh;
+}
+__device__ __forceinline__ int64_t query_row(const AttnArgs& a, int row) {
+  const int t = a.by_group(row);
+  return t * a.q_sn + (int64_t)(row - t * a.group) * a.q_sh;
 }
 
 // Tiles before each line (of one item; first[lines]: all) and keys of each line, by the CTA's first 128 threads; every thread calls it.
-__device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int* first, int* keys, int* warp_sum) {
+__device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int* first, int* keys, uint8_t* lasts, int* warp_sum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int PER = (MAX_LINES + 1 + 127) / 128;
   int before = 0, mine[PER];
@@ -126,7 +157,11 @@ __device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int
   for (int u = 0; u < PER; ++u) {
     const int line = tid * PER + u;
     int m = 0;
-    if (line < a.lines) keys[line] = m = keys_of(a, a.line0 + line);
+    if (line < a.lines) {
+      int last;
+      keys[line] = m = keys_of(a, a.line0 + line, last);
+      lasts[line] = (uint8_t)last;
+    }
     mine[u] = before;
     before += (m + tile_keys - 1) / tile_keys;
   }
@@ -148,25 +183,27 @@ __device__ __forceinline__ void scan_lines(const AttnArgs& a, int tile_keys, int
 
 template <typename T, int D>
 __device__ __forceinline__ void empty_line(const AttnArgs& a, int line) {
-  const int b = a.by_n(line), i = line - b * a.n;
-  uint4* o = reinterpret_cast<uint4*>((T*)a.o + (int64_t)line * a.H * D);
-  for (int e = threadIdx.x; e < a.H * D / 8; e += blockDim.x) o[e] = make_uint4(0, 0, 0, 0);
-  for (int h = threadIdx.x; h < a.H; h += blockDim.x) a.lse[((int64_t)b * a.H + h) * a.n + i] = -INFINITY;
+  const int b = a.by_packs(line), i0 = (line - b * a.packs) * a.pack, tokens = min(a.pack, a.n - i0);
+  uint4* o = reinterpret_cast<uint4*>((T*)a.o + ((int64_t)b * a.n + i0) * a.H * D);
+  for (int e = threadIdx.x; e < tokens * a.H * D / 8; e += blockDim.x) o[e] = make_uint4(0, 0, 0, 0);
+  for (int e = threadIdx.x; e < tokens * a.H; e += blockDim.x) a.lse[((int64_t)b * a.H + e / tokens) * a.n + i0 + e % tokens] = -INFINITY;
 }
 
 // This CTA's part [begin, end) of the list of tiles, and the place of its first; lines without keys get their outputs here.  With clusters, its part of
 // one item's tiles: line 0 of what it sees, which is line `line0` of the call.  Every thread calls it.
 template <typename T, int D, bool CLUSTER>
-__device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int* first, int* keys, int* warp_sum, int items, int& begin, int& end, int& line0) {
+__device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int* first, int* keys, uint8_t* lasts, int* warp_sum, int items, int& begin, int& end, int& line0) {
   const int tid = threadIdx.x;
   if constexpr (CLUSTER) {
     const int unit = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster, line = unit / items;
     line0 = line;
-    const int m = keys_of(a, line), tiles = (m + tile_keys - 1) / tile_keys, share = (tiles + a.cluster - 1) / a.cluster;
+    int last;
+    const int m = keys_of(a, line, last), tiles = (m + tile_keys - 1) / tile_keys, share = (tiles + a.cluster - 1) / a.cluster;
     if (tid == 0) {
       first[0] = 0;
       first[1] = tiles;
       keys[0] = m;
+      lasts[0] = (uint8_t)last;
     }
     __syncthreads();
     begin = min(rank * share, tiles);
@@ -175,7 +212,7 @@ __device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int*
     return Walk{0, unit % items, begin, tiles};
   } else {
     line0 = a.line0;
-    scan_lines(a, tile_keys, first, keys, warp_sum);
+    scan_lines(a, tile_keys, first, keys, lasts, warp_sum);
     const int total = first[a.lines] * items;
     const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
     begin = min((int)blockIdx.x * per, total);
@@ -208,18 +245,16 @@ __device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int*
 // the result or as a part.  `join`: all four warps are here and see what each wrote to shared memory; false: one gave up.
 template <typename T, int D, int APART, bool CLUSTER, typename W, typename J>
 __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* stat, float* sums, const Walk& at, const int* first, int items, int begin, int end,
-                                            bool last, int line0, float* cluster_sums, float2* cluster_stat, J join) {
+                                            bool last, int line0, int keys, int last_token, float* cluster_sums, float2* cluster_stat, J join) {
   constexpr int ROWS = W::ROWS, ROUNDS = W::ROUNDS, WIDTH = D / ROUNDS, LANES = 128 / ROWS;     // threads of a row
   static_assert(APART >= ROWS * WIDTH, "floats from one warp's sums to the next's");
   static_assert(WIDTH % (4 * LANES) == 0, "whole columns");
   const int tid = threadIdx.x, warp = tid >> 5;
   w.statistics(stat + warp * ITEM_ROWS);
-  const int b = a.by_n(line0 + at.line), i = line0 + at.line - b * a.n;
-  const int h = a.by_blocks(at.item), block = at.item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
   const int item_begin = first[at.line] * items + at.item * at.tiles, item_end = item_begin + at.tiles;
   const bool whole = !CLUSTER && item_begin >= begin && item_end <= end;
   const int row = tid / LANES;
-  const int64_t out = ((int64_t)(line0 + at.line) * a.H + h * a.group + block * ITEM_ROWS + row) * D;
+  const RowAt ra = row_at(a, line0 + at.line, at.item, row, keys, last_token);
   const int slot = 2 * blockIdx.x + (item_begin <= begin ? 0 : 1);
   float part[4], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -232,8 +267,8 @@ __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* sta
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float2 st = stat[x * ITEM_ROWS + row];
-        part[x] = st.x == -INFINITY ? -1.f : fast_exp2(st.x - m);
-        if (!(part[x] < 0.f)) l = fmaf(part[x], st.y, l);
+        part[x] = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m);       // (its sums are zeros, or NaN)
+        l = fmaf(part[x], st.y, l);
       }
     }
     if (!join()) return false;
@@ -247,31 +282,30 @@ __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* sta
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float4 f = *reinterpret_cast<const float4*>(sums + x * APART + row * WIDTH + (col ^ W::turn(row)));
-        if (!(part[x] < 0.f)) {
-          v.x = fmaf(part[x], f.x, v.x);
-          v.y = fmaf(part[x], f.y, v.y);
-          v.z = fmaf(part[x], f.z, v.z);
-          v.w = fmaf(part[x], f.w, v.w);
-        }
+        v.x = fmaf(part[x], f.x, v.x);
+        v.y = fmaf(part[x], f.y, v.y);
+        v.z = fmaf(part[x], f.z, v.z);
+        v.w = fmaf(part[x], f.w, v.w);
       }
     }
     // (a cluster's part may lie where the sums did)
     if (CLUSTER && !join()) return false;
-    if (row < rows) {
+    if (ra.there) {
 #pragma unroll
       for (int j = 0; j < WIDTH / (4 * LANES); ++j) {
         const int col = (tid % LANES) * 4 + 4 * LANES * j;
         const float4 v = vs[j];
         if (whole)
-          *reinterpret_cast<uint2*>((T*)a.o + out + y * WIDTH + col) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+          *reinterpret_cast<uint2*>((T*)a.o + ra.o * D + y * WIDTH + col) =
+              ra.empty ? make_uint2(0, 0) : make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
         else if (CLUSTER)
           *reinterpret_cast<float4*>(cluster_sums + row * D + y * WIDTH + col) = v;
         else
           *reinterpret_cast<float4*>(a.part + ((int64_t)slot * ITEM_ROWS + row) * D + y * WIDTH + col) = v;
       }
     }
-    if (y == 0 && row < rows && tid % LANES == 0) {
-      if (whole) a.lse[((int64_t)b * a.H + h * a.group + block * ITEM_ROWS + row) * a.n + i] = (m + log2f(l)) * LN2;
+    if (y == 0 && ra.there && tid % LANES == 0) {
+      if (whole) a.lse[ra.lse] = ra.empty ? -INFINITY : (m + log2f(l)) * LN2;
       else if (CLUSTER) cluster_stat[row] = make_float2(m, l);
       else a.part_stat[slot * ITEM_ROWS + row] = make_float2(m, l);
     }
@@ -291,22 +325,22 @@ __device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
 }
 
 // End of an item that a cluster shares: each CTA joins its share of the rows from all CTAs' parts, read over distributed shared memory.  The first four warps of every
-// CTA call it, those of a CTA without keys, too (stat -inf); no CTA leaves before the others have read its part.
+// CTA call it, those of a CTA without keys, too (a negative denominator); no CTA leaves before the others have read its part.
 template <typename T, int D>
-__device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* sums, const float2* stat, int line, int item) {
+__device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* sums, const float2* stat, int line, int item, int keys, int last) {
   cluster_sync();
   const int tid = threadIdx.x, rank = blockIdx.x % a.cluster;
-  const int b = a.by_n(line), i = line - b * a.n;
-  const int h = a.by_blocks(item), block = item - h * a.blocks, rows = min(a.group - block * ITEM_ROWS, ITEM_ROWS);
   constexpr int LANES = D / 4;                 // threads of a row, four columns each
-  for (int row = rank + a.cluster * (tid / LANES); row < rows; row += a.cluster * (128 / LANES)) {
+  for (int row = rank + a.cluster * (tid / LANES); row < min(a.pack * a.group, ITEM_ROWS); row += a.cluster * (128 / LANES)) {
+    const RowAt ra = row_at(a, line, item, row, keys, last);
+    if (!ra.there) continue;
     const int col = tid % LANES * 4;
     float m = -INFINITY, l = 0.f;
     float2 st[8];
     float4 f[8];
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      st[x] = make_float2(-INFINITY, 0.f);
+      st[x] = make_float2(-INFINITY, -1.f);
       if (x >= a.cluster) continue;
       asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(st[x].x), "=f"(st[x].y) : "r"(cluster_at(stat + row, x)));
       asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[x].x), "=f"(f[x].y), "=f"(f[x].z), "=f"(f[x].w) : "r"(cluster_at(sums + row * D + col, x)));
@@ -316,8 +350,8 @@ __device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* s
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      if (st[x].x == -INFINITY) continue;
-      const float w = fast_exp2(st[x].x - m);
+      if (st[x].y < 0.f) continue;
+      const float w = st[x].x == -INFINITY ? 0.f : fast_exp2(st[x].x - m);
       l = fmaf(w, st[x].y, l);
       v.x = fmaf(w, f[x].x, v.x);
       v.y = fmaf(w, f[x].y, v.y);
@@ -325,15 +359,14 @@ __device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* s
       v.w = fmaf(w, f[x].w, v.w);
     }
     const float inv = 1.f / l;
-    const int head = h * a.group + block * ITEM_ROWS + row;
-    *reinterpret_cast<uint2*>((T*)a.o + ((int64_t)line * a.H + head) * D + col) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-    if (col == 0) a.lse[((int64_t)b * a.H + head) * a.n + i] = (m + log2f(l)) * LN2;
+    *reinterpret_cast<uint2*>((T*)a.o + ra.o * D + col) = ra.empty ? make_uint2(0, 0) : make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+    if (col == 0) a.lse[ra.lse] = ra.empty ? -INFINITY : (m + log2f(l)) * LN2;
   }
   cluster_sync();
 }
 
 // Kernels of 4-bit rows: CTAs of an SM, keys of a tile, and the launch of one kernel.
-int attn4_resident(int d, int group);
+int attn4_resident(int d, int rows);
 int attn4_launch(AttnArgs a, int dtype, int d, int ctas, cudaStream_t st);
 
 }  // namespace ha

@@ -29,7 +29,7 @@ struct Stage4 {
   static constexpr int QF = (NQ == 2 ? D * 32 : 0) + (1 + G) * ROWS * 4;   // a warp's query operands (16 rows); units and sums of the queries
   static constexpr int WARP = NS * BYTES + QF + NS * 16 + 64;          // of a warp, too: what its stages hold, and its place in the list
   static constexpr int PARTS = ROWS * (D * 4 + 8);           // with clusters: the CTA's part
-  static constexpr int SMEM = 4 * WARP + PARTS + 4 * ITEM_ROWS * 8 + (2 * MAX_LINES + 8) * 4 + 32;
+  static constexpr int SMEM = 4 * WARP + PARTS + 4 * ITEM_ROWS * 8 + (2 * MAX_LINES + 8) * 4 + 32 + MAX_LINES;
   static constexpr int ROUNDS = NQ;                          // in which the warps' sums are joined: column ranges that fit a stage
   static_assert(ROWS * D / ROUNDS * 4 <= BYTES, "a warp's sums fit a stage");
   static_assert(WK * ROW == 2048 && WK * SC == 256 && WARP % 16 == 0, "copies of a warp's rows and scales");
@@ -57,7 +57,7 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, bool PACKED>
 struct Worker4 {
   using S = Stage4<D, NQ>;
   static constexpr int G = S::G, ROWS = S::ROWS, ROUNDS = S::ROUNDS, STEPS = D / 16, NB = S::NB, KW = S::KW;
@@ -79,8 +79,9 @@ struct Worker4 {
 
   // Query operands: fp16, every query times the power of two that brings its largest element to 2^13 .. 2^14.  Lane c of a query's four holds elements
   // 16 c .. 16 c + 15 of each group, paired as the codes come out of their words: (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
-  __device__ __forceinline__ void begin(const AttnArgs& a, const uint8_t* q, int rows) {
+  __device__ __forceinline__ void begin(const AttnArgs& a, int line, int item) {
     const int c = lane & 3;
+    const uint8_t* q = query_of(a, line, item);
     v_top = 0x1p-24f;
     limit = -INFINITY;
     uint32_t f[STEPS][2 * NQ];
@@ -88,13 +89,15 @@ struct Worker4 {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int row = lane / 4 + 8 * n;
+      const bool there = row_at(a, line, item, row).there;
+      const uint8_t* from = q + (there ? query_row(a, row) : 0);
       float x[G][16], top = 0.f, s[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         s[g] = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint4 w = row < rows ? *reinterpret_cast<const uint4*>(q + row * a.q_sh + (8 * g + 2 * c + u) * 16) : make_uint4(0, 0, 0, 0);
+          const uint4 w = there ? *reinterpret_cast<const uint4*>(from + (8 * g + 2 * c + u) * 16) : make_uint4(0, 0, 0, 0);
           const uint32_t ws[4] = {w.x ^ a.flip, w.y ^ a.flip, w.z ^ a.flip, w.w ^ a.flip};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -206,8 +209,8 @@ struct Worker4 {
     }
   }
 
-  // KW keys of a tile from this warp's key `base` on, of which the first `left` exist.
-  __device__ __forceinline__ void keys(const uint8_t* stage, int base, int left) {
+  // KW keys of a tile from this warp's key `base` on, of which the line's last token, the `last`-th of its pack, sees the first `left`.
+  __device__ __forceinline__ void keys(const AttnArgs& a, const uint8_t* stage, int base, int left, int last) {
     const int c = lane & 3, r = lane >> 2;
     const uint8_t *kp = stage + k_at + base * S::ROW, *sp = stage + s_at + base * S::SC, *vp = stage + v_at + base * S::ROW;
     constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
@@ -269,14 +272,21 @@ struct Worker4 {
         }
       }
     }
-    if (left < KW) {
+    const bool mixed = left - last < KW;
+    if (mixed) {
 #pragma unroll
-      for (int blk = 0; blk < NB; ++blk)
+      for (int n = 0; n < NQ; ++n) {
+        const int sees[2] = {left - keys_short<PACKED>(a, 8 * n + 2 * c, last), left - keys_short<PACKED>(a, 8 * n + 2 * c + 1, last)};
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-          if (blk * 16 + y * 8 + key_of(r) >= left)
+        for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) x[blk][y][n] = pack_f2(-INFINITY, -INFINITY);
+          for (int y = 0; y < 2; ++y) {
+            const int key = blk * 16 + y * 8 + key_of(r);
+            float u, v;
+            unpack_f2(x[blk][y][n], u, v);
+            x[blk][y][n] = pack_f2(key < sees[0] ? u : -INFINITY, key < sees[1] ? v : -INFINITY);
+          }
+      }
     }
     float top = -INFINITY;
 #pragma unroll
@@ -325,9 +335,17 @@ struct Worker4 {
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
             float u, v;
+            uint64_t mids = dup_f2(m);
             unpack_f2(fmul2(p[n], dup_f2(f.x)), u, v);
+            if (PACKED && mixed) {            // (a group that stands for no number counts for the queries that see its key, and for no others)
+              float pu, pv;
+              unpack_f2(p[n], pu, pv);
+              if (pu == 0.f) u = 0.f;
+              if (pv == 0.f) v = 0.f;
+              mids = pack_f2(pu == 0.f ? 0.f : m, pv == 0.f ? 0.f : m);
+            }
             pb[g][n][y] = transposed(pack2<__half>(u, v));
-            offset[g][n] = ffma2(p[n], dup_f2(m), offset[g][n]);
+            offset[g][n] = ffma2(p[n], mids, offset[g][n]);
           }
         }
       }
@@ -418,7 +436,7 @@ struct alignas(16) Place {
   int keys;
 };
 
-template <typename T, int D, int NQ, bool CLUSTER>
+template <typename T, int D, int NQ, bool CLUSTER, bool PACKED>
 __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel(const __grid_constant__ AttnArgs a) {
   using S = Stage4<D, NQ>;
   constexpr int NS = S::NS, TK = S::TK, KW = S::KW, WK = S::WK;
@@ -431,6 +449,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
   int* keys = first + MAX_LINES + 4;                                         // [lines]
   const uint32_t join_bar = smem_u32(keys + MAX_LINES);
   int* warp_sum = keys + MAX_LINES + 2;                                      // [4]
+  uint8_t* lasts = reinterpret_cast<uint8_t*>(warp_sum + 4);                 // [lines]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int items = a.Hk * a.blocks;
   if (tid == 0) {
@@ -441,7 +460,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
   if (CLUSTER) chain_release();              // (as in paged_attn.cu: the kernel behind is let in at the end, or at once)
   chain_wait();
   int begin, end, line0;
-  const Walk start = take_part<T, D, CLUSTER>(a, TK, first, keys, warp_sum, items, begin, end, line0);
+  const Walk start = take_part<T, D, CLUSTER>(a, TK, first, keys, lasts, warp_sum, items, begin, end, line0);
   const int lines = CLUSTER ? 1 : a.lines;
   if (begin >= end && (!CLUSTER || keys[0] == 0)) return;
 
@@ -451,7 +470,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
   const uint32_t base = smem_u32(mine);
   auto settle = [&](const Walk& f) {
     const int h = a.by_blocks(f.item);
-    place->table = a.c.table + a.by_n(line0 + f.line) * a.c.table_sb;
+    place->table = a.c.table + a.by_packs(line0 + f.line) * a.c.table_sb;
     place->head = h * a.c.sh;
     place->head_s = h * a.c.ssh;
     place->keys = keys[f.line];
@@ -514,7 +533,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     __syncwarp();
   };
 
-  Worker4<T, D, NQ> w;
+  Worker4<T, D, NQ, PACKED> w;
   w.lane = lane;
   w.qs = reinterpret_cast<uint4*>(mine + NS * S::BYTES);
   w.q_unit = reinterpret_cast<float*>(mine + NS * S::BYTES + (NQ == 2 ? D * 32 : 0));
@@ -546,15 +565,17 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     __syncwarp();
     const int4 t = what[s];
     if (it == begin || t.w == 0) {
-      const int b = a.by_n(line0 + t.y), i = line0 + t.y - b * a.n, h = a.by_blocks(t.z), block = t.z - h * a.blocks;
-      w.begin(a, a.q + b * a.q_sb + i * a.q_sn + (int64_t)(h * a.group + block * ITEM_ROWS) * a.q_sh, min(a.group - block * ITEM_ROWS, ITEM_ROWS));
+      w.begin(a, line0 + t.y, t.z);
     }
+    const int last = PACKED ? lasts[t.y] : 0;
     if (t.x < WK) w.clear_tail(stage, t.x);
 #pragma unroll
-    for (int y = 0; y < WK; y += KW) w.keys(stage, y, t.x - y);
+    for (int y = 0; y < WK; y += KW) w.keys(a, stage, y, t.x - y, last);
     if (t.x + warp * WK <= TK || it == end - 1) {
       const Walk at = {t.y, t.z, t.w, first[t.y + 1] - first[t.y]};
-      ok = finish_item<T, D, S::WARP / 4, CLUSTER>(a, w, stat, reinterpret_cast<float*>(smem + s * S::BYTES), at, first, items, begin, end, it == end - 1, line0, cluster_sums, cluster_stat, join) && join();
+      ok = finish_item<T, D, S::WARP / 4, CLUSTER>(a, w, stat, reinterpret_cast<float*>(smem + s * S::BYTES), at, first, items, begin, end, it == end - 1, line0, keys[t.y],
+                                                              last, cluster_sums, cluster_stat, join) &&
+           join();
       if (!ok) break;
     }
     __syncwarp();
@@ -564,10 +585,10 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
   }
   if constexpr (CLUSTER) {
     if (begin >= end || !ok) {
-      if (tid < S::ROWS) cluster_stat[tid] = make_float2(-INFINITY, 0.f);
+      if (tid < S::ROWS) cluster_stat[tid] = make_float2(-INFINITY, -1.f);
     }
     __syncwarp();
-    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, start.item);
+    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, start.item, keys[0], lasts[0]);
   }
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   cp_async_wait<0>();
@@ -577,31 +598,38 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
 template <typename T, int D, int NQ>
 int launch4(const AttnArgs& a, int ctas, cudaStream_t st) {
   using S = Stage4<D, NQ>;
-  if (a.cluster > 0) {
-    HA_SMEM_ATTR_ONCE((paged_attn4_kernel<T, D, NQ, true>), S::SMEM, "ha_paged_attn");
-    launch_chained_clusters(paged_attn4_kernel<T, D, NQ, true>, ctas, 128, S::SMEM, a.cluster, st, a);
-  } else {
-    HA_SMEM_ATTR_ONCE((paged_attn4_kernel<T, D, NQ, false>), S::SMEM, "ha_paged_attn");
-    launch_chained(paged_attn4_kernel<T, D, NQ, false>, ctas, 128, S::SMEM, st, a);
-  }
+  auto launch = [&](auto kernel) {
+    if (a.cluster > 0) launch_chained_clusters(kernel, ctas, 128, S::SMEM, a.cluster, st, a);
+    else launch_chained(kernel, ctas, 128, S::SMEM, st, a);
+  };
+#define HA_PAGED_VARIANT(cluster, packed)                                                          \
+  do {                                                                                             \
+    HA_SMEM_ATTR_ONCE((paged_attn4_kernel<T, D, NQ, cluster, packed>), S::SMEM, "ha_paged_attn");  \
+    launch(paged_attn4_kernel<T, D, NQ, cluster, packed>);                                         \
+  } while (0)
+  if (a.cluster > 0 && a.pack > 1) HA_PAGED_VARIANT(true, true);
+  else if (a.cluster > 0) HA_PAGED_VARIANT(true, false);
+  else if (a.pack > 1) HA_PAGED_VARIANT(false, true);
+  else HA_PAGED_VARIANT(false, false);
+#undef HA_PAGED_VARIANT
   HA_LAUNCHED("ha_paged_attn");
   return HA_OK;
 }
 
 }  // namespace
 
-int attn4_resident(int d, int group) {
-  if (d == 128) return group > 8 ? Stage4<128, 2>::CTAS : Stage4<128, 1>::CTAS;
-  return group > 8 ? Stage4<64, 2>::CTAS : Stage4<64, 1>::CTAS;
+int attn4_resident(int d, int rows) {
+  if (d == 128) return rows > 8 ? Stage4<128, 2>::CTAS : Stage4<128, 1>::CTAS;
+  return rows > 8 ? Stage4<64, 2>::CTAS : Stage4<64, 1>::CTAS;
 }
 
 int attn4_launch(AttnArgs a, int dtype, int d, int ctas, cudaStream_t st) {
-  const bool bf = dtype == HA_BF16;
+  const bool bf = dtype == HA_BF16, many = a.group * a.pack > 8;
   if (d == 128) {
-    if (a.group > 8) return bf ? launch4<__nv_bfloat16, 128, 2>(a, ctas, st) : launch4<__half, 128, 2>(a, ctas, st);
+    if (many) return bf ? launch4<__nv_bfloat16, 128, 2>(a, ctas, st) : launch4<__half, 128, 2>(a, ctas, st);
     return bf ? launch4<__nv_bfloat16, 128, 1>(a, ctas, st) : launch4<__half, 128, 1>(a, ctas, st);
   }
-  if (a.group > 8) return bf ? launch4<__nv_bfloat16, 64, 2>(a, ctas, st) : launch4<__half, 64, 2>(a, ctas, st);
+  if (many) return bf ? launch4<__nv_bfloat16, 64, 2>(a, ctas, st) : launch4<__half, 64, 2>(a, ctas, st);
   return bf ? launch4<__nv_bfloat16, 64, 1>(a, ctas, st) : launch4<__half, 64, 1>(a, ctas, st);
 }
 

@@ -32,7 +32,7 @@ def _ext():
     """The operators' host side (csrc/paged_ext.cpp: checks, allocations and the call into the library), loaded once."""
     global _EXT
     if _EXT is None:
-        if not os.path.exists(os.path.join(os.path.dirname(L.LIB_PATH), '_paged_ext.so')):
+        if not os.path.exists(os.path.join(os.path.dirname(__file__), '_paged_ext.so')):
             raise RuntimeError('_paged_ext.so is missing: build it with `python hyperattention_b200/csrc/build.py` (there is no fallback implementation)')
         from . import _paged_ext
         lib = L.load()

@@ -233,6 +233,41 @@ def test_attention_values_that_are_no_numbers(bits):
     assert (o.double() - want)[ok].abs().max() < 0.05
 
 
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('dtype', [BF, HF])
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('H,Hk,n', [(1, 1, 16), (2, 2, 5), (6, 2, 4), (8, 1, 3), (16, 4, 9), (5, 1, 17)])
+def test_attention_tokens_share_an_item(bits, dtype, d, H, Hk, n):
+    """packs of neighbouring tokens: whole and broken ones, sequences shorter than a pack, padding inside one"""
+    attend_case(bits, dtype, d, H, Hk, 16, [n, 1, 0, 200 + n, 64, 3], n=n)
+    attend_case(bits, dtype, d, H, Hk, 16, [n, 1, 9, 200 + n, 64, 3000], n=n, counts=[n, 1, 2, n - 1, 0, n])
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('what', [math.nan, math.inf])
+@pytest.mark.parametrize('d', [64, 128])
+def test_attention_tokens_of_an_item_keep_apart(bits, what, d):
+    """a value that is no number in the last keys reaches the tokens that see its key, and no others, where they share an item"""
+    g = torch.Generator().manual_seed(15)
+    n, H, Hk = 8, 2, 1
+    for length in (8, 70, 129):
+        for back in (1, 3, 7):
+            rk, rv = [[torch.randn(length, Hk, d, generator=g)] for _ in 'kv']
+            rv[0][length - back, 0, 5] = what
+            cache, table, ks, vs = make_cache(rk, rv, 16, bits, BF, g)
+            q = torch.randn(1, n, H, d, generator=g).to(BF).cuda()
+            o, lse = ha.paged_attn_func(q, cache, table, torch.tensor([length], dtype=torch.int32, device='cuda'))
+            want, wl = reference(q, ks, vs, [length], [n], d ** -0.5)[:2]
+            assert torch.equal(torch.isfinite(o), torch.isfinite(want)) and o[0, :n - back].isfinite().all() and not o[0, n - back:, :, 5].isfinite().any()
+            ok = torch.isfinite(want)
+            assert (o.double() - want)[ok].abs().max() < 0.05 and (lse.double() - wl).abs().max() < 1e-4
+            # ... and a key
+            rk[0][length - back, 0, 5] = what
+            cache, table, ks, vs = make_cache(rk, rv, 16, bits, BF, g)
+            o, lse = ha.paged_attn_func(q, cache, table, torch.tensor([length], dtype=torch.int32, device='cuda'))
+            assert lse[0, :, :n - back].isfinite().all() and o[0, :n - back].isfinite().all() and o[0, n - back:, :, 5].isnan().all()
+
+
 def test_attention_no_numbers_in_a_whole_warp():
     """NaN scores through all the keys of a warp's part, beside finite ones"""
     g = torch.Generator().manual_seed(5)
