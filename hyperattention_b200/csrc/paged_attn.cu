@@ -233,7 +233,7 @@ struct Worker {
 };
 
 // The warp that fetches: tiles begin .. end - 1 into the ring.  full[s]: every lane arrives once its copies are there; empty[s]: the four warps that compute.
-template <int D, bool CLUSTER>
+template <int D, bool CLUSTER, bool PACKED>
 __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, const int* first, const int* keys, Walk at,
                                             int begin, int end, int items, int line0, uint32_t base, uint32_t bars, int* abort_flag) {
   using S = Stage<D>;
@@ -275,8 +275,8 @@ __device__ __forceinline__ void fetch_tiles(const AttnArgs& a, const CUtensorMap
 #pragma unroll
       for (int e = lane; e < ITEM_ROWS * C; e += 32) {
         const int r = e / C, chunk = e % C;
-        const bool there = row_at(a, line0 + at.line, at.item, r).there;
-        cp_async16(dst + S::Q + r * 2 * D + chunk_at(r, chunk) * 16, q + (there ? query_row(a, r) : 0) + chunk * 16, there ? 16 : 0);
+        const bool there = row_at<PACKED>(a, line0 + at.line, at.item, r).there;
+        cp_async16(dst + S::Q + r * 2 * D + chunk_at(r, chunk) * 16, q + (there ? query_row<PACKED>(a, r) : 0) + chunk * 16, there ? 16 : 0);
       }
     }
     cp_async_arrive(full);
@@ -319,17 +319,20 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     mbar_init(bars + 8 * 2 * NS, 4);
     mbar_fence_init();
     *abort_flag = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&km) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vm) : "memory");
   }
   // The kernel behind is let in at the end: its CTAs would take the places that come free one by one, several on some SMs and none on others
   // (1 x 131072 tokens, 32 heads x 64, passes back to back: 242 us with an early release, 165 without).
   if (CLUSTER) chain_release();              // (short kernels, fewer CTAs than there is room for: the next one may be placed at once)
   chain_wait();
+  // (parts of one tile would be as many to join as tiles: 1 x 8000 tokens, two K/V heads: 15.5 us, 12.5 with parts of two)
   int begin, end, line0;
-  Walk at = take_part<T, D, CLUSTER>(a, TK, first, keys, lasts, warp_sum, items, begin, end, line0);
+  Walk at = take_part<T, D, CLUSTER>(a, TK, 2, first, keys, lasts, warp_sum, items, begin, end, line0);
   const int lines = CLUSTER ? 1 : a.lines, item = at.item;
   if (begin >= end && (!CLUSTER || keys[0] == 0)) return;
   if (warp == 4) {
-    if (begin < end) fetch_tiles<D, CLUSTER>(a, &km, &vm, first, keys, at, begin, end, items, line0, base, bars, abort_flag);
+    if (begin < end) fetch_tiles<D, CLUSTER, PACKED>(a, &km, &vm, first, keys, at, begin, end, items, line0, base, bars, abort_flag);
     if (CLUSTER) {                             // (these threads count in the cluster's barriers)
       __syncwarp();
       cluster_sync();
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     w.tile(a, stage, left, last);
     const bool ends = at.tile == at.tiles - 1 || it == end - 1;
     if (ends) {
-      ok = finish_item<T, D, 16 * D, CLUSTER>(a, w, stat, reinterpret_cast<float*>(stage), at, first, items, begin, end, it == end - 1, line0, keys[at.line], last, cluster_sums, cluster_stat,
+      ok = finish_item<T, D, 16 * D, CLUSTER, PACKED>(a, w, stat, reinterpret_cast<float*>(stage), at, first, items, begin, end, it == end - 1, line0, keys[at.line], last, cluster_sums, cluster_stat,
                                               join);
       if (!ok) break;
     }
@@ -380,36 +383,37 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
       if (tid < ITEM_ROWS) cluster_stat[tid] = make_float2(-INFINITY, -1.f);
     }
     __syncwarp();
-    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, item, keys[0], lasts[0]);
+    cluster_finish<T, D, PACKED>(a, cluster_sums, cluster_stat, line0, item, keys[0], lasts[0]);
   }
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   chain_release();
 }
 
-// Joins the parts of the items that cross from one CTA's list to the next.  Block (c, row): the item that begins in CTA c's list and ends behind it.
+// Joins the parts of the items that cross from one CTA's list to the next.  Block (c, y): rows 4 y .. of the item that begins in CTA c's list and ends behind it;
+// four warps a row, each every fourth part.
+constexpr int COMBINE_ROWS = 2;
 template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const AttnArgs a) {
-  __shared__ float red[4][D];
-  __shared__ float red_m[4], red_l[4];
+__global__ void __launch_bounds__(128 * COMBINE_ROWS) paged_combine_kernel(const __grid_constant__ AttnArgs a) {
+  __shared__ float red[COMBINE_ROWS][4][D];
+  __shared__ float red_m[COMBINE_ROWS][4], red_l[COMBINE_ROWS][4];
   chain_wait();
-  const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int c = blockIdx.x, sub = threadIdx.x / 128, row = blockIdx.y * COMBINE_ROWS + sub, tid = threadIdx.x % 128, warp = tid >> 5, lane = tid & 31;
   const int total = a.meta[0], per = a.meta[1];
   if ((int64_t)(c + 1) * per >= total) return;
   const int4 hd = a.head[c];
   if (hd.y <= (c + 1) * per || hd.x < c * per) return;                 // ends here, or began before
   int token;
   const int keys = keys_of(a, hd.z, token);
-  const RowAt ra = row_at(a, hd.z, hd.w, row, keys, token);
-  if (!ra.there) return;
-  const int last = (hd.y - 1) / per, pieces = last - c + 1;
+  const RowAt ra = row_at<true>(a, hd.z, hd.w, row, keys, token);
+  const int last = (hd.y - 1) / per, pieces = ra.there ? last - c + 1 : 0;
   auto slot = [&](int p) { return 2 * (c + p) + (p == 0 && hd.x > c * per ? 1 : 0); };
   float m = -INFINITY;
   for (int p = tid; p < pieces; p += 128) m = fmaxf(m, a.part_stat[slot(p) * ITEM_ROWS + row].x);
 #pragma unroll
   for (int s = 1; s < 32; s *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  if (lane == 0) red_m[warp] = m;
+  if (lane == 0) red_m[sub][warp] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+  m = fmaxf(fmaxf(red_m[sub][0], red_m[sub][1]), fmaxf(red_m[sub][2], red_m[sub][3]));
   // pieces p = warp, warp + 4, ...: a lane D / 32 columns
   constexpr int E = D / 32;
   float v[E], l = 0.f;
@@ -427,19 +431,19 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const AttnArgs a) {
       const float2 f = *reinterpret_cast<const float2*>(src);
       y[0] = f.x, y[1] = f.y;
     }
-    {
-      const float w = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m);
-      l = fmaf(w, st.y, l);
+    const float w = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m);
+    l = fmaf(w, st.y, l);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = fmaf(w, y[e], v[e]);
-    }
+    for (int e = 0; e < E; ++e) v[e] = fmaf(w, y[e], v[e]);
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) red[warp][lane * E + e] = v[e];
-  if (lane == 0) red_l[warp] = l;
+  for (int e = 0; e < E; ++e) red[sub][warp][lane * E + e] = v[e];
+  if (lane == 0) red_l[sub][warp] = l;
   __syncthreads();
-  l = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
-  if (tid < D) ((T*)a.o)[ra.o * D + tid] = from_f32<T>(ra.empty ? 0.f : ((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) / l);
+  if (!ra.there) return;
+  l = (red_l[sub][0] + red_l[sub][1]) + (red_l[sub][2] + red_l[sub][3]);
+  const float(*r)[D] = red[sub];
+  if (tid < D) ((T*)a.o)[ra.o * D + tid] = from_f32<T>(ra.empty ? 0.f : ((r[0][tid] + r[1][tid]) + (r[2][tid] + r[3][tid])) / l);
   if (tid == 0) a.lse[ra.lse] = ra.empty ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
@@ -608,13 +612,13 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
     else rc = bf ? launch_attn<__nv_bfloat16, 128>(a, p, now, st) : launch_attn<__half, 128>(a, p, now, st);
     if (rc != HA_OK) return rc;
     if (now == 1 || cluster > 0) continue;
-    const dim3 grid(now - 1, attn_rows(p) < ITEM_ROWS ? attn_rows(p) : ITEM_ROWS);
+    const dim3 grid(now - 1, ((attn_rows(p) < ITEM_ROWS ? attn_rows(p) : ITEM_ROWS) + COMBINE_ROWS - 1) / COMBINE_ROWS);
     if (p.d == 64) {
-      if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 64>, grid, 128, 0, st, a);
-      else launch_chained(paged_combine_kernel<__half, 64>, grid, 128, 0, st, a);
+      if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 64>, grid, 128 * COMBINE_ROWS, 0, st, a);
+      else launch_chained(paged_combine_kernel<__half, 64>, grid, 128 * COMBINE_ROWS, 0, st, a);
     } else {
-      if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 128>, grid, 128, 0, st, a);
-      else launch_chained(paged_combine_kernel<__half, 128>, grid, 128, 0, st, a);
+      if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 128>, grid, 128 * COMBINE_ROWS, 0, st, a);
+      else launch_chained(paged_combine_kernel<__half, 128>, grid, 128 * COMBINE_ROWS, 0, st, a);
     }
     HA_LAUNCHED("ha_paged_attn");
   }

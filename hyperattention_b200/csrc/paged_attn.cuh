@@ -127,10 +127,11 @@ struct RowAt {
   int64_t o, lse;                     // its outputs: a row of o, an element of lse
   bool there, empty;                  // one of the call's rows; one of padding, or without keys
 };
-// (keys, last: what keys_of says of the line)
+// (keys, last: what keys_of says of the line; PACKED: items of several tokens)
+template <bool PACKED>
 __device__ __forceinline__ RowAt row_at(const AttnArgs& a, int line, int item, int row, int keys = 1, int last = 0) {
   const int b = a.by_packs(line), i0 = (line - b * a.packs) * a.pack, h = a.by_blocks(item), block = item - h * a.blocks;
-  const int t = a.by_group(row), of_group = block * ITEM_ROWS + row - t * a.group, i = i0 + t, head = h * a.group + of_group;
+  const int t = PACKED ? a.by_group(row) : 0, of_group = block * ITEM_ROWS + row - t * a.group, i = i0 + t, head = h * a.group + of_group;
   RowAt r;
   r.there = t < a.pack && i < a.n && of_group < a.group;
   r.empty = t > last || keys <= last - t;
@@ -143,8 +144,9 @@ __device__ __forceinline__ const uint8_t* query_of(const AttnArgs& a, int line, 
   const int b = a.by_packs(line), i0 = (line - b * a.packs) * a.pack, h = a.by_blocks(item), block = item - h * a.blocks;
   return a.q + b * a.q_sb + i0 * a.q_sn + (int64_t)(h * a.group + block * ITEM_ROWS) * a.q_sh;
 }
+template <bool PACKED>
 __device__ __forceinline__ int64_t query_row(const AttnArgs& a, int row) {
-  const int t = a.by_group(row);
+  const int t = PACKED ? a.by_group(row) : 0;
   return t * a.q_sn + (int64_t)(row - t * a.group) * a.q_sh;
 }
 
@@ -190,9 +192,9 @@ __device__ __forceinline__ void empty_line(const AttnArgs& a, int line) {
 }
 
 // This CTA's part [begin, end) of the list of tiles, and the place of its first; lines without keys get their outputs here.  With clusters, its part of
-// one item's tiles: line 0 of what it sees, which is line `line0` of the call.  Every thread calls it.
+// one item's tiles: line 0 of what it sees, which is line `line0` of the call.  `least`: tiles of a part, at least.  Every thread calls it.
 template <typename T, int D, bool CLUSTER>
-__device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int* first, int* keys, uint8_t* lasts, int* warp_sum, int items, int& begin, int& end, int& line0) {
+__device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int least, int* first, int* keys, uint8_t* lasts, int* warp_sum, int items, int& begin, int& end, int& line0) {
   const int tid = threadIdx.x;
   if constexpr (CLUSTER) {
     const int unit = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster, line = unit / items;
@@ -214,7 +216,7 @@ __device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int*
     line0 = a.line0;
     scan_lines(a, tile_keys, first, keys, lasts, warp_sum);
     const int total = first[a.lines] * items;
-    const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+    const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, least);
     begin = min((int)blockIdx.x * per, total);
     end = min(begin + per, total);
     if (blockIdx.x == 0 && tid == 0) {
@@ -243,7 +245,7 @@ __device__ __forceinline__ Walk take_part(const AttnArgs& a, int tile_keys, int*
 
 // End of an item, or of this CTA's part of it: the sums of the four warps that compute are joined through `sums` (a stage that has been read), and go out as
 // the result or as a part.  `join`: all four warps are here and see what each wrote to shared memory; false: one gave up.
-template <typename T, int D, int APART, bool CLUSTER, typename W, typename J>
+template <typename T, int D, int APART, bool CLUSTER, bool PACKED, typename W, typename J>
 __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* stat, float* sums, const Walk& at, const int* first, int items, int begin, int end,
                                             bool last, int line0, int keys, int last_token, float* cluster_sums, float2* cluster_stat, J join) {
   constexpr int ROWS = W::ROWS, ROUNDS = W::ROUNDS, WIDTH = D / ROUNDS, LANES = 128 / ROWS;     // threads of a row
@@ -254,7 +256,7 @@ __device__ __forceinline__ bool finish_item(const AttnArgs& a, W& w, float2* sta
   const int item_begin = first[at.line] * items + at.item * at.tiles, item_end = item_begin + at.tiles;
   const bool whole = !CLUSTER && item_begin >= begin && item_end <= end;
   const int row = tid / LANES;
-  const RowAt ra = row_at(a, line0 + at.line, at.item, row, keys, last_token);
+  const RowAt ra = row_at<PACKED>(a, line0 + at.line, at.item, row, keys, last_token);
   const int slot = 2 * blockIdx.x + (item_begin <= begin ? 0 : 1);
   float part[4], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -326,13 +328,13 @@ __device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
 
 // End of an item that a cluster shares: each CTA joins its share of the rows from all CTAs' parts, read over distributed shared memory.  The first four warps of every
 // CTA call it, those of a CTA without keys, too (a negative denominator); no CTA leaves before the others have read its part.
-template <typename T, int D>
+template <typename T, int D, bool PACKED>
 __device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* sums, const float2* stat, int line, int item, int keys, int last) {
   cluster_sync();
   const int tid = threadIdx.x, rank = blockIdx.x % a.cluster;
   constexpr int LANES = D / 4;                 // threads of a row, four columns each
   for (int row = rank + a.cluster * (tid / LANES); row < min(a.pack * a.group, ITEM_ROWS); row += a.cluster * (128 / LANES)) {
-    const RowAt ra = row_at(a, line, item, row, keys, last);
+    const RowAt ra = row_at<PACKED>(a, line, item, row, keys, last);
     if (!ra.there) continue;
     const int col = tid % LANES * 4;
     float m = -INFINITY, l = 0.f;

@@ -89,8 +89,8 @@ struct Worker4 {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int row = lane / 4 + 8 * n;
-      const bool there = row_at(a, line, item, row).there;
-      const uint8_t* from = q + (there ? query_row(a, row) : 0);
+      const bool there = row_at<PACKED>(a, line, item, row).there;
+      const uint8_t* from = q + (there ? query_row<PACKED>(a, row) : 0);
       float x[G][16], top = 0.f, s[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
   if (CLUSTER) chain_release();              // (as in paged_attn.cu: the kernel behind is let in at the end, or at once)
   chain_wait();
   int begin, end, line0;
-  const Walk start = take_part<T, D, CLUSTER>(a, TK, first, keys, lasts, warp_sum, items, begin, end, line0);
+  const Walk start = take_part<T, D, CLUSTER>(a, TK, 1, first, keys, lasts, warp_sum, items, begin, end, line0);
   const int lines = CLUSTER ? 1 : a.lines;
   if (begin >= end && (!CLUSTER || keys[0] == 0)) return;
 
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     for (int y = 0; y < WK; y += KW) w.keys(a, stage, y, t.x - y, last);
     if (t.x + warp * WK <= TK || it == end - 1) {
       const Walk at = {t.y, t.z, t.w, first[t.y + 1] - first[t.y]};
-      ok = finish_item<T, D, S::WARP / 4, CLUSTER>(a, w, stat, reinterpret_cast<float*>(smem + s * S::BYTES), at, first, items, begin, end, it == end - 1, line0, keys[t.y],
+      ok = finish_item<T, D, S::WARP / 4, CLUSTER, PACKED>(a, w, stat, reinterpret_cast<float*>(smem + s * S::BYTES), at, first, items, begin, end, it == end - 1, line0, keys[t.y],
                                                               last, cluster_sums, cluster_stat, join) &&
            join();
       if (!ok) break;
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
       if (tid < S::ROWS) cluster_stat[tid] = make_float2(-INFINITY, -1.f);
     }
     __syncwarp();
-    cluster_finish<T, D>(a, cluster_sums, cluster_stat, line0, start.item, keys[0], lasts[0]);
+    cluster_finish<T, D, PACKED>(a, cluster_sums, cluster_stat, line0, start.item, keys[0], lasts[0]);
   }
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   cp_async_wait<0>();
