@@ -5,6 +5,7 @@
 namespace ha {
 
 constexpr int PAGED_GROUP = 64;      // elements that share a scale in a 4-bit row
+constexpr long long PAGED_MOST = 0x7fffffffLL - 65536;      // positions of a sequence: 32-bit numbers, with room for a tile behind the last
 
 // What every entry point of the cache asks of its arguments.
 inline int paged_check(const ha_paged_params& p) {
@@ -12,7 +13,7 @@ inline int paged_check(const ha_paged_params& p) {
   if ((p.bits != 16 && p.bits != 4) || (p.d != 64 && p.d != 128)) return HA_ERR_INVALID;
   if (p.B < 0 || p.n < 0 || p.Hk < 1 || p.H < 0 || p.H % p.Hk != 0) return HA_ERR_INVALID;
   if (p.pages < 0 || p.page_size < 1 || p.columns < 0 || p.table_sb < 0) return HA_ERR_INVALID;
-  if ((long long)p.columns * p.page_size > 0x7fffffffLL) return HA_ERR_TOO_LARGE;       // positions are 32-bit
+  if ((long long)p.columns * p.page_size > PAGED_MOST) return HA_ERR_TOO_LARGE;
   if (p.page_sp < 0 || p.page_sh < 0 || p.page_st < 0 || p.scale_sp < 0 || p.scale_sh < 0 || p.scale_st < 0) return HA_ERR_INVALID;
   if (p.B > 0 && (!p.lengths || (p.columns > 0 && !p.table))) return HA_ERR_INVALID;
   if (p.pages > 0) {

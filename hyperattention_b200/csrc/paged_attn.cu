@@ -13,7 +13,8 @@
 // Here: 16-bit rows, the joining of parts, the entry points.  (4-bit rows: paged_attn4.cu.)  A CTA: four warps that compute, each a quarter of a tile's
 // keys with its own running maximum and sums, which are joined at the item's end; and one that fetches tiles into a ring of NS stages, across
 // items, by tensor copies (128-byte swizzle; boxes of as many rows as both a page and a tile are made of, so that any page size will do).
-// 1 x 131072 tokens, 32 heads x 64: 165 us, 6.5 TB/s.
+// 1 x 131072 tokens, 32 heads x 64: 167 us, 6.4 TB/s (98 % of a copy's rate).  Batch of 32 x up to 8192, two K/V heads x 128: 27.6 us, 3.5 TB/s: what remains is the
+// latency of a kernel's start, of a part's end and of the joining.
 #include <string.h>
 
 #include <numeric>
@@ -48,7 +49,7 @@ struct Stage {
 template <int TK>
 __device__ __forceinline__ uint32_t slab_at(int row, int chunk) { return (chunk >> 3) * (TK * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 
-template <typename T, int D, bool PACKED>
+template <typename T, int D, bool CLUSTER, bool PACKED>
 struct Worker {
   using S = Stage<D>;
   static constexpr int ROWS = 16, ROUNDS = 1;
@@ -108,20 +109,21 @@ struct Worker {
     __syncwarp();
   }
 
-  // Where the tokens of a pack see different keys: is there a value among this warp's rows of V that is no number?  Weight 0 would not take it out.
-  __device__ __forceinline__ bool infinite(const uint8_t* stage) const {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr uint32_t EXP = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    bool found = false;
-    for (int e = lane; e < S::KW * (D / 8); e += 32) {
-      const uint4 v = lds128(stage + S::V + slab_at<S::TK>(warp * S::KW + e / (D / 8), e % (D / 8)));
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  // Is there an infinity or a NaN among the values of V that the products take?  The second number of a weight, zero or negative, would make a NaN of an infinity;
+  // and where the tokens of a pack see different keys, weight 0 would not take one out.  (Zero times the values, added up: 0 or NaN.)
+  static __device__ __forceinline__ bool infinite(const uint32_t (&b)[D / 16][4]) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const uint32_t zero = 0;
+    const T2 none = *reinterpret_cast<const T2*>(&zero);
+    T2 found[4] = {none, none, none, none};
 #pragma unroll
-      for (int y = 0; y < 4; ++y) found = found || (w[y] & EXP) == EXP || ((w[y] >> 16) & EXP) == EXP;
-    }
-    return __any_sync(0xffffffffu, found);
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) found[y] = __hfma2(*reinterpret_cast<const T2*>(&b[j][y]), none, found[y]);
+    const T2 all = __hadd2(__hadd2(found[0], found[1]), __hadd2(found[2], found[3]));
+    return __any_sync(0xffffffffu, (*reinterpret_cast<const uint32_t*>(&all) & 0x7fff7fffu) != 0);
   }
-  // ... then each row takes the values of the keys that it sees, one by one.
+  // ... then each row takes the values of the keys that it sees, one by one, by weights in 32 bits.
   __device__ __forceinline__ void add_singly(const AttnArgs& a, const uint8_t* stage, int left, int last, const float (&p)[NT][4]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
     const int sees[2] = {left - keys_short<PACKED>(a, lane >> 2, last), left - keys_short<PACKED>(a, (lane >> 2) + 8, last)};
@@ -164,6 +166,13 @@ struct Worker {
       mma16816<T>(x[0], qf[ks], b[0], b[1]);
       mma16816<T>(x[1], qf[ks], b[2], b[3]);
     }
+    // V's fragments before the weights are known, so that their latency is hidden; kept to the products with clusters, loaded once more in the list's kernel, where their
+    // registers cost spills (tokens of a batch of 32 x 8192, kept: 29.8 us, loaded again: 27.6; of 16 x 4096 by clusters, appended, too: 15.5 and 17.3).
+    uint32_t v[D / 16][4];
+    const int vrow = warp * S::KW + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) ldmatrix4t(v[j], at + S::V + slab_at<S::TK>(vrow, 2 * j + (lane >> 4)));
+    const bool singly = infinite(v);
     if (left - last < S::KW) {
       const int sees[2] = {left - keys_short<PACKED>(a, lane >> 2, last), left - keys_short<PACKED>(a, (lane >> 2) + 8, last)};
 #pragma unroll
@@ -191,19 +200,17 @@ struct Worker {
         hi[2 * t + r] = w;
         lo[2 * t + r] = pack2<T>(p0 - f.x, p1 - f.y);
       }
-    const int vrow = warp * S::KW + (lane & 15);
-    if (PACKED && last > 0 && left > 0 && left - last < S::KW && infinite(stage)) {
+    if (singly) {
       add_singly(a, stage, left, last, x);
       return;
     }
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
-      uint32_t b[4];
-      ldmatrix4t(b, at + S::V + slab_at<S::TK>(vrow, 2 * j + (lane >> 4)));
-      mma16816<T>(acc[2 * j], hi, b[0], b[1]);
-      mma16816<T>(acc[2 * j + 1], hi, b[2], b[3]);
-      mma16816<T>(acc[2 * j], lo, b[0], b[1]);
-      mma16816<T>(acc[2 * j + 1], lo, b[2], b[3]);
+      if (!CLUSTER) ldmatrix4t(v[j], at + S::V + slab_at<S::TK>(vrow, 2 * j + (lane >> 4)));
+      mma16816<T>(acc[2 * j], hi, v[j][0], v[j][1]);
+      mma16816<T>(acc[2 * j + 1], hi, v[j][2], v[j][3]);
+      mma16816<T>(acc[2 * j], lo, v[j][0], v[j][1]);
+      mma16816<T>(acc[2 * j + 1], lo, v[j][2], v[j][3]);
     }
   }
 
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     return;
   }
 
-  Worker<T, D, PACKED> w;
+  Worker<T, D, CLUSTER, PACKED> w;
   const uint32_t join_bar = bars + 8 * 2 * NS;
   uint32_t joined = 0;
   auto join = [&]() {
@@ -385,12 +392,13 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     __syncwarp();
     cluster_finish<T, D, PACKED>(a, cluster_sums, cluster_stat, line0, item, keys[0], lasts[0]);
   }
+  if (!ok && !CLUSTER && tid == 0) a.head[blockIdx.x] = make_int4(0, 0, 0, 0);       // nothing to join from here
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   chain_release();
 }
 
-// Joins the parts of the items that cross from one CTA's list to the next.  Block (c, y): rows 4 y .. of the item that begins in CTA c's list and ends behind it;
-// four warps a row, each every fourth part.
+// Joins the parts of the items that cross from one CTA's list to the next.  Block (c, y): rows COMBINE_ROWS y .. of the item that begins in CTA c's list and ends behind
+// it; four warps a row, each every fourth part.  Latency alone: a chain of four loads, about 4 us (rows a block: two, 28.4 us for a batch of 32 x 8192 with its attention; four, 29.5).
 constexpr int COMBINE_ROWS = 2;
 template <typename T, int D>
 __global__ void __launch_bounds__(128 * COMBINE_ROWS) paged_combine_kernel(const __grid_constant__ AttnArgs a) {
@@ -470,8 +478,9 @@ int attn_ctas(const ha_paged_params& p, int lines) {
 }
 
 // CTAs that share an item as a cluster, or 0.  Short contexts and few items: a cluster joins its parts over distributed shared memory, without a workspace and a
-// second launch (1 x 515 tokens: 8.1 -> 5.5 us on the device, 7 -> 4 us of host time).  Every item gets the same CTAs, however long it is, so that the list of tiles,
-// which deals them out evenly, is for what takes longer than the joining.
+// second launch (1 x 515 tokens, two K/V heads: 8.2 -> 6.9 us on the device, 7.1 -> 2.7 us for the call).  Every item gets the same CTAs, however long it is, so that
+// the list of tiles, which deals them out evenly, is for what takes longer than the joining: at CLUSTER_TILES 4 a batch of 16 x 4096 goes by the list, 16.9 us for 15.4; at
+// 20, 1 x 8000 goes by clusters of 8, 19.5 us for 12.5; at 40 a batch of 32 x 8192, 37 us for 28.
 int attn_cluster(const ha_paged_params& p) {
   const int64_t units = p.B * attn_packs(p) * attn_items(p);
   const int64_t tiles = ((int64_t)p.columns * p.page_size + attn_tile(p) - 1) / attn_tile(p), resident = (int64_t)sm_count() * attn_resident(p);
@@ -528,7 +537,8 @@ int launch_attn(const AttnArgs& a, const ha_paged_params& p, int ctas, cudaStrea
 int attn_check(const ha_paged_params& p) {
   const int rc = paged_check(p);
   if (rc != HA_OK) return rc;
-  if (p.H < 1 || p.scale == 0.f) return HA_ERR_INVALID;
+  // (by a scale below that the room above a reference, SLACK / scale, would be infinite)
+  if (p.H < 1 || !(fabsf(p.scale) >= 0x1p-100f) || isinf(p.scale)) return HA_ERR_INVALID;
   if ((int64_t)p.B * p.n > 0x7fffffffLL - 65536 || (int64_t)p.H * p.d > 1 << 24) return HA_ERR_TOO_LARGE;
   if (p.B > 0 && p.n > 0 && attn_lines(p) < 1) return HA_ERR_TOO_LARGE;
   return HA_OK;
@@ -560,7 +570,7 @@ int64_t ha_paged_attn_workspace_bytes(const ha_paged_params* pp) {
   const ha_paged_params& p = *pp;
   if ((p.bits != 16 && p.bits != 4) || (p.d != 64 && p.d != 128) || p.B < 0 || p.n < 0 || p.Hk < 1 || p.H < 1 || p.H % p.Hk != 0 || p.columns < 0 || p.page_size < 1)
     return HA_ERR_INVALID;
-  if ((int64_t)p.columns * p.page_size > 0x7fffffffLL) return HA_ERR_TOO_LARGE;
+  if ((int64_t)p.columns * p.page_size > PAGED_MOST) return HA_ERR_TOO_LARGE;
   const int64_t all = p.B * attn_packs(p), lines = attn_lines(p);
   if (all == 0 || attn_cluster(p) > 0) return 0;
   return lines < 1 ? (int64_t)HA_ERR_TOO_LARGE : attn_workspace(p, attn_ctas(p, (int)lines));

@@ -305,7 +305,7 @@ struct Worker4 {
       for (int y = 0; y < 2; ++y) {
         load_words(sp + S::VS + (16 * blk + 8 * y) * S::SC, vs[blk][y]);
 #pragma unroll
-        for (int g = 0; g < G; ++g) most = __hmax2(most, *reinterpret_cast<const __half2*>(&vs[blk][y][g]));
+        for (int g = 0; g < G; ++g) most = __hmax2(most, __habs2(*reinterpret_cast<const __half2*>(&vs[blk][y][g])));
       }
     const float step = __low2float(most);
     if (__any_sync(0xffffffffu, top > limit || step >= v_top)) raise(x, step);
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
       if (left > 0) {
         const int col = a.c.by_page(key0), slot = key0 - col * a.c.page_size, page = f.table[col];
         if (paged_checked(a.c, page)) {
-          const int64_t off = page * a.c.sp + f.head + slot * S::ROW + lane * 16, off_s = page * a.c.ssp + f.head_s + slot * S::SC + (lane & 15) * 16;
+          const int64_t off = page * a.c.sp + f.head + (int64_t)slot * S::ROW + lane * 16, off_s = page * a.c.ssp + f.head_s + (int64_t)slot * S::SC + (lane & 15) * 16;
           const uint8_t *k = a.c.k + off, *v = a.c.v + off, *sc = (lane < 16 ? a.c.ks : a.c.vs) + off_s;
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
@@ -590,6 +590,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     __syncwarp();
     cluster_finish<T, D, PACKED>(a, cluster_sums, cluster_stat, line0, start.item, keys[0], lasts[0]);
   }
+  if (!ok && !CLUSTER && tid == 0) a.head[blockIdx.x] = make_int4(0, 0, 0, 0);       // nothing to join from here
   if (!ok && lane == 0) report_timeout(a.c.status, a.c.status_host);
   cp_async_wait<0>();
   chain_release();

@@ -268,6 +268,33 @@ def test_attention_tokens_of_an_item_keep_apart(bits, what, d):
             assert lse[0, :, :n - back].isfinite().all() and o[0, :n - back].isfinite().all() and o[0, n - back:, :, 5].isnan().all()
 
 
+@pytest.mark.parametrize('dtype', [BF, HF])
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('n', [1, 4, 16])
+def test_attention_infinite_values(dtype, d, n):
+    """an infinity among the values that a row sees is the column's sum, of its own sign, whatever its weight's rounding: of the first key, of equal weights, ..."""
+    g = torch.Generator().manual_seed(25)
+    for length in (1, 17, 200, 3000):
+        for even in (True, False):
+            rk, rv = [[torch.randn(length, 1, d, generator=g)] for _ in 'kv']
+            if even:
+                rk[0].zero_()
+            rv[0][0, 0, 3], rv[0][length // 2, 0, 4], rv[0][length - 1, 0, 5] = math.inf, -math.inf, math.inf
+            rv[0][length // 3, 0, 6], rv[0][length // 4, 0, 6] = math.inf, -math.inf if length > 4 else math.inf
+            cache, table, ks, vs = make_cache(rk, rv, 16, 16, dtype, g)
+            q = torch.randn(1, n, 2, d, generator=g).to(dtype).cuda()
+            o, lse = ha.paged_attn_func(q, cache, table, torch.tensor([length], dtype=torch.int32, device='cuda'))
+            want, wl = reference(q, ks, vs, [length], [n], d ** -0.5)[:2]
+            empty = (wl == -math.inf).transpose(1, 2)
+            assert not o[empty].any() and torch.equal(lse == -math.inf, wl == -math.inf)
+            seen, whole = o[~empty].double(), want[~empty]
+            assert torch.equal(seen.isnan(), whole.isnan()) and torch.equal(seen.isinf(), whole.isinf())
+            assert torch.equal(seen[whole.isinf()], whole[whole.isinf()])
+            # |o| < 8, as all values are: half a step is 4 eps at most, and the rest (weights in 16 bits or more, sums in 32) far below
+            ok = whole.isfinite()
+            assert (seen - whole)[ok].abs().max() < 8 * torch.finfo(dtype).eps
+
+
 def test_attention_no_numbers_in_a_whole_warp():
     """NaN scores through all the keys of a warp's part, beside finite ones"""
     g = torch.Generator().manual_seed(5)
@@ -338,6 +365,33 @@ def test_attention_beyond_32_bits_of_elements():
     check(o, lse, reference(q, [x], [x], [200], [1], d ** -0.5), 16, BF, d, 200)
     k, v = ha.paged_gather(cache, table, held + 200, 201)
     assert torch.equal(k[0, 0, :200], rows[0, :, 0]) and torch.equal(k, v) and not k[0, 0, 200:].any()
+
+
+def test_four_bits_beyond_32_bits_of_a_page():
+    """one page whose rows lie past 2^31 bytes of it: appended, attended to, in whole runs"""
+    page, d = 2 ** 25 + 128, 128
+    codes, scales = [torch.zeros(1, 1, page, d // 2, dtype=torch.uint8, device='cuda') for _ in 'kv'], [torch.zeros(1, 1, page, 2, 2, dtype=HF, device='cuda') for _ in 'kv']
+    cache = ha.PagedCache(*codes, *scales)
+    g = torch.Generator().manual_seed(2)
+    held, new, lead = 2 ** 25 + 10, 100, 2 ** 25 + 10
+    table, i32 = torch.zeros(1, 1, dtype=torch.int32, device='cuda'), lambda x: torch.tensor([x], dtype=torch.int32, device='cuda')
+    q = torch.randn(1, 1, 16, d, generator=g).to(BF).cuda()
+    # keys along the sum of the queries: scores that outweigh the millions of zeros
+    k = (q.float().sum(2, keepdim=True).cpu() + 0.5 * torch.randn(1, new, 1, d, generator=g)).to(BF).cuda()
+    v = torch.randn(1, new, 1, d, generator=g).to(BF).cuda()
+    ha.paged_append(cache, k, v, table, i32(held))
+    o, lse = ha.paged_attn_func(q, cache, table, i32(held + new), softmax_scale=0.25)
+    kk, vv = dequantised(k[0]), dequantised(v[0])
+    s = torch.einsum('hd,ld->hl', q[0, 0].double(), kk[:, 0]) * 0.25                       # [heads, new]; all other scores and values are 0
+    z = torch.logaddexp(torch.logsumexp(s, -1), torch.full((16,), math.log(lead), dtype=F64, device='cuda'))
+    p = (s - z[:, None]).exp()
+    want = p @ vv[:, 0]
+    assert s.max() > 20 and (p.sum(-1) > 0.5).any()
+    e = 8 * (d + 8) * 2 ** -24 * torch.einsum('hd,ld->hl', q[0, 0].double().abs(), kk[:, 0].abs()).amax(-1) * 0.25
+    # as in check(): the score's error, the weights' rounding beside 7.5 steps (of spans below 8), chains of 2^25 / (128 * 400) tiles of additions
+    tol = 2 ** -9 * want.abs() + (2 * e + 2 ** -11 + 1200 * 2 ** -23)[:, None] * 8
+    assert ((o[0, 0].double() - want).abs() <= tol).all()
+    assert ((lse[0, :, 0].double() - z).abs() <= e + 2 ** -22 * (z.abs() + 32) + 1200 * 2 ** -23).all()
 
 
 # ---------------------------------------------------------------------------------------------------------------------

@@ -1,5 +1,6 @@
 """The paged key/value cache without a GPU: what the handle and the C entry points refuse (no kernel is launched), and the 4-bit row format."""
 import ctypes as C
+import math
 import os
 
 import pytest
@@ -37,7 +38,7 @@ def _params(**over):
 
 BAD = [(dict(dtype=L.FP32), -2), (dict(dtype=9), -2), (dict(bits=8), -1), (dict(d=96), -1), (dict(d=0), -1), (dict(B=-1), -1), (dict(n=-1), -1),
        (dict(Hk=0), -1), (dict(H=7), -1), (dict(pages=-1), -1), (dict(page_size=0), -1), (dict(columns=-1), -1),
-       (dict(columns=1 << 20, page_size=1 << 20), -5), (dict(lengths=None), -1), (dict(table=None), -1), (dict(k_pages=None), -1), (dict(v_pages=None), -1),
+       (dict(columns=1 << 20, page_size=1 << 20), -5), (dict(columns=2 ** 31 - 1, page_size=1), -5), (dict(columns=1, page_size=2 ** 31 - 1), -5), (dict(lengths=None), -1), (dict(table=None), -1), (dict(k_pages=None), -1), (dict(v_pages=None), -1),
        (dict(k_pages=264), -1), (dict(page_st=100), -1), (dict(page_sp=-4096), -1), (dict(bits=4, k_scales=None), -1), (dict(bits=4, v_scales=260), -1),
        (dict(bits=4, scale_st=2), -1), (dict(bits=4, page_st=72), -1)]
 
@@ -55,7 +56,8 @@ def test_entry_points_refuse_their_own(lib):
     for over in (dict(k=None), dict(v=None), dict(q=None), dict(q_out=None), dict(k_out=264), dict(rope=256, rot=3), dict(rope=256, rot=130),
                  dict(rope=256, rot=64, rope_dtype=L.FP16), dict(rope=256, rot=64, rope_rows=-1)):
         assert lib.ha_paged_append(C.byref(_params(**over)), None) == -1, over
-    for over in (dict(q=None), dict(o=None), dict(lse=None), dict(q=264), dict(q_sh=100), dict(H=0)):
+    for over in (dict(q=None), dict(o=None), dict(lse=None), dict(q=264), dict(q_sh=100), dict(H=0), dict(scale=0.0), dict(scale=math.nan),
+                 dict(scale=math.inf), dict(scale=-math.inf), dict(scale=1e-38)):
         assert lib.ha_paged_attn(C.byref(_params(**over)), None) == -1, over
     assert lib.ha_paged_attn(C.byref(_params(columns=4000)), None) == -3                        # workspace too small
     assert lib.ha_paged_attn(C.byref(_params(workspace=None, columns=4000)), None) == -3
