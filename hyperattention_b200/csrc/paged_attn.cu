@@ -479,8 +479,8 @@ int attn_ctas(const ha_paged_params& p, int lines) {
 
 // CTAs that share an item as a cluster, or 0.  Short contexts and few items: a cluster joins its parts over distributed shared memory, without a workspace and a
 // second launch (1 x 515 tokens, two K/V heads: 8.2 -> 6.9 us on the device, 7.1 -> 2.7 us for the call).  Every item gets the same CTAs, however long it is, so that
-// the list of tiles, which deals them out evenly, is for what takes longer than the joining: at CLUSTER_TILES 4 a batch of 16 x 4096 goes by the list, 16.9 us for 15.4; at
-// 20, 1 x 8000 goes by clusters of 8, 19.5 us for 12.5; at 40 a batch of 32 x 8192, 37 us for 28.
+// the list of tiles, which deals them out evenly, is for what takes longer than the joining: with CLUSTER_TILES 7 a batch of 16 x 4096 goes by the list, 17.4 us for 15.3 (1 x 5000 gains:
+// 12.1 for 13.6); with 20, 1 x 8000 by clusters of 8, 19.5 us for 12.5; with 40 a batch of 32 x 8192, 37 us for 28.
 int attn_cluster(const ha_paged_params& p) {
   const int64_t units = p.B * attn_packs(p) * attn_items(p);
   const int64_t tiles = ((int64_t)p.columns * p.page_size + attn_tile(p) - 1) / attn_tile(p), resident = (int64_t)sm_count() * attn_resident(p);

@@ -163,8 +163,9 @@ def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
     counts   int32 [B] or None: rows of q that are tokens of the sequence, n of each without it
 
     Row i < counts[b] sees positions 0 .. lengths[b] - counts[b] + i.  A row that sees none, and padding rows, have o = 0 and lse = -inf.  Consecutive
-    query heads share a K/V head.  Every token reads the sequence's keys again (from the L2 cache where they fit): made for one to a few
-    tokens a sequence; prompts belong to HyperAttention or flash_attn_func."""
+    query heads share a K/V head.  Keys are read once for 16 query rows of a K/V head, those of neighbouring tokens where a token has fewer, and again
+    for the next 16: made for one to a few tokens a sequence; prompts belong to HyperAttention or flash_attn_func.  Over a cache in 4 bits,
+    queries of 1e34 and more are not told from infinite ones."""
     return _call('attn', cache, q, table, lengths, counts, float(softmax_scale or cache.head_dim ** -0.5))
 
 

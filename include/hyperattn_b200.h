@@ -343,7 +343,8 @@ int ha_paged_maps(const ha_paged_params* p, void* maps);
 int ha_paged_append(const ha_paged_params* p, void* stream);
 
 /* Query row i < counts[b] attends to positions 0 .. lengths[b] - counts[b] + i: lengths counts the rows of this call, too.  o and natural-log lse as
- * the other attention entry points give them; a row without keys, and rows i >= counts[b], have o = 0, lse = -infinity.  q on 16-byte rows. */
+ * the other attention entry points give them; a row without keys, and rows i >= counts[b], have o = 0, lse = -infinity.  q on 16-byte rows.  |scale|
+ * between 2^-100 and infinity.  The workspace may be 0 bytes (short contexts: the parts are joined within a cluster of CTAs). */
 int64_t ha_paged_attn_workspace_bytes(const ha_paged_params* p);
 int ha_paged_attn(const ha_paged_params* p, void* stream);
 
