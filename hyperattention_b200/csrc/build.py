@@ -43,7 +43,7 @@ def build_ext(force=False, verbose=False):
                os.path.join(cuda, 'include')]
     cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC', '-I' + os.path.join(ROOT, 'include')] + ['-isystem' + i for i in include] + \
         [f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', src, '-o', EXT, '-L' + os.path.join(base, 'lib'),
-         '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lc10', '-lc10_cuda']
+         '-ltorch', '-ltorch_cpu', '-ltorch_cuda', '-ltorch_python', '-lc10', '-lc10_cuda']
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or r.returncode != 0:
         sys.stderr.write(' '.join(cmd) + '\n' + r.stdout + r.stderr)

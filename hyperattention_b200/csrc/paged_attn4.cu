@@ -29,7 +29,8 @@ struct Stage4 {
   static constexpr int KW = 16 * NB, TK = attn4_tile(D), WK = TK / 4;      // those keys; keys of a tile, a warp's of them
   static constexpr int ROW = D / 2, G = D / PAGED_GROUP, SC = 4 * G, ROWS = 8 * NQ;        // bytes of a row, of its scales; queries
   static constexpr int V = WK * ROW, KS = 2 * WK * ROW, VS = KS + WK * SC, BYTES = VS + WK * SC;       // a warp's stage
-  static constexpr int CTAS = D == 128 ? 3 : 4, NS = 2;
+  // (16 rows x 128: 170 registers a thread; for a fourth CTA sums would be spilled, 80 -> 107 us at 64 x 32768 tokens.  8 rows gain by it: 59.0 -> 57.1)
+  static constexpr int CTAS = D == 128 && NQ == 2 ? 3 : 4, NS = 2;
   static constexpr int QF = (NQ == 2 ? D * 32 : 0) + (1 + G) * ROWS * 4;   // a warp's query operands (16 rows); units and sums of the queries
   static constexpr int WARP = NS * BYTES + QF + NS * 16 + 64;          // of a warp, too: what its stages hold, and its place in the list
   static constexpr int PARTS = ROWS * (D * 4 + 8);           // with clusters: the CTA's part

@@ -1,6 +1,7 @@
 // The Python operators of the paged cache, in C++: argument checks, allocations and the call into the C ABI.  A step of generation is a few short calls a
 // block; written in Python, one took 13 us of host time where the kernels take 7.  The kernels themselves are reached through the C ABI alone, whose
 // functions this module is handed (init): it links to neither the library nor CUDA's tools.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -82,7 +83,8 @@ void want_rows(const Handle& h, const Tensor& t, int64_t B, int64_t n, int64_t h
 // rows that are not contiguous are copied, as in HyperAttention
 Tensor rows(const Tensor& t) { return t.dim() == 0 || t.size(t.dim() - 1) <= 1 || t.stride(t.dim() - 1) == 1 ? t : t.contiguous(); }
 
-Tensor dense(const Handle& h, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, at::TensorOptions().dtype(type).device(h.device)); }
+// (at::empty without its way through the dispatcher)
+Tensor dense(const Handle& h, at::IntArrayRef shape, at::ScalarType type) { return at::detail::empty_cuda(shape, type, h.device, std::nullopt); }
 
 int run(int (*fn)(const ha_paged_params*, void*), const Handle& h, const ha_paged_params& p) {
   c10::cuda::OptionalCUDAGuard guard;
