@@ -69,7 +69,6 @@ __device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t mask, uint32_t 
   asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(a), "r"(mask), "r"(flip));
   return r;
 }
-__device__ __forceinline__ uint64_t dup_f2(float v) { return pack_f2(v, v); }
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));

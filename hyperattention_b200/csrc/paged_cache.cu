@@ -121,28 +121,37 @@ __device__ __forceinline__ uint2 quantise(const float (&x)[PART], __half2& scale
   // the nearest number open, or the offset's own rounding puts an extreme out of the range, and there alone, the quotient itself is taken.
   const float inv = __fdividef(1.f, s), low = -m * inv, magic = 12582912.f;      // 1.5 * 2^23: adding it rounds to a whole number
   const float open = 0.5f - (fabsf(low) + 16.f) * 0x1p-20f;
-  float c[PART], off = 0.f;
+  float off = 0.f;
+  uint64_t c[PART / 2];              // pairs of neighbours
 #pragma unroll
-  for (int j = 0; j < PART; j += 2) {
-    const float t = fmaf(x[j], inv, low), u = fmaf(x[j + 1], inv, low);
-    c[j] = __fsub_rn(__fadd_rn(t, magic), magic);
-    c[j + 1] = __fsub_rn(__fadd_rn(u, magic), magic);
-    off = fmax3(off, fabsf(t - c[j]), fabsf(u - c[j + 1]));
+  for (int j = 0; j < PART / 2; ++j) {
+    const uint64_t t = ffma2(pack_f2(x[2 * j], x[2 * j + 1]), dup_f2(inv), dup_f2(low));
+    c[j] = fadd2(fadd2(t, dup_f2(magic)), dup_f2(-magic));
+    float u, v;
+    unpack_f2(ffma2(c[j], dup_f2(-1.f), t), u, v);
+    off = fmax3(off, fabsf(u), fabsf(v));
   }
   if (off > open || fmaf(hi, inv, low) > 15.25f || fmaf(lo, inv, low) < -0.25f) {
 #pragma unroll
-    for (int j = 0; j < PART; ++j) c[j] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], m), s)), 0.f), 15.f);
+    for (int j = 0; j < PART / 2; ++j) {
+      const float u = rintf(__fdiv_rn(__fsub_rn(x[2 * j], m), s)), v = rintf(__fdiv_rn(__fsub_rn(x[2 * j + 1], m), s));
+      c[j] = pack_f2(fminf(fmaxf(u, 0.f), 15.f), fminf(fmaxf(v, 0.f), 15.f));
+    }
   }
   // (sums of four codes are whole numbers below 2^16)
   uint32_t w[4];
 #pragma unroll
-  for (int y = 0; y < 4; ++y) w[y] = (uint32_t)fmaf(fmaf(fmaf(c[4 * y + 3], 16.f, c[4 * y + 2]), 16.f, c[4 * y + 1]), 16.f, c[4 * y]);
+  for (int y = 0; y < 4; ++y) {
+    float u, v;
+    unpack_f2(ffma2(c[2 * y + 1], dup_f2(256.f), c[2 * y]), u, v);
+    w[y] = (uint32_t)fmaf(v, 16.f, u);
+  }
   return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 
 // One block a token, D / 16 lanes a row, sixteen elements a lane, which keeps its cosines and sines for all the heads that it meets; two rows of a
 // lane under way at once.  Bound by the bytes of q, k and v for prompts, by the chain length -> page -> store for single tokens.  32768 tokens, 32 + 2 + 2
-// heads x 128: 108 us, 5.7 TB/s; 2 x 8191 tokens, 32 + 32 + 32 heads x 64, into 4 bits: 95 us, where the codes' arithmetic is as long as the copies; one token of 32
+// heads x 128: 108 us, 5.7 TB/s; 2 x 8191 tokens, 32 + 32 + 32 heads x 64, into 4 bits: 92 us, issue-bound by the codes' arithmetic (half of it in pairs: 95 us without); one token of 32
 // sequences: 2.3 us.  (Launch bounds for 5, 6 or 8 blocks of an SM spill or gain nothing.)
 template <typename T, int D, int BITS, bool WIDE>
 __global__ void __launch_bounds__(128) paged_append_kernel(const AppendArgs a) {
