@@ -17,6 +17,7 @@
 // latency of a kernel's start, of a part's end and of the joining.
 #include <string.h>
 
+#include <algorithm>
 #include <numeric>
 #include <type_traits>
 
@@ -397,15 +398,15 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
   chain_release();
 }
 
-// Joins the parts of the items that cross from one CTA's list to the next.  Block (c, y): rows COMBINE_ROWS y .. of the item that begins in CTA c's list and ends behind
-// it; four warps a row, each every fourth part.  Latency alone: a chain of four loads, about 4 us (rows a block: two, 28.4 us for a batch of 32 x 8192 with its attention; four, 29.5).
-constexpr int COMBINE_ROWS = 2;
-template <typename T, int D>
-__global__ void __launch_bounds__(128 * COMBINE_ROWS) paged_combine_kernel(const __grid_constant__ AttnArgs a) {
-  __shared__ float red[COMBINE_ROWS][4][D];
-  __shared__ float red_m[COMBINE_ROWS][4], red_l[COMBINE_ROWS][4];
+// Joins the parts of the items that cross from one CTA's list to the next.  Block (c, y): rows ROWS y .. of the item that begins in CTA c's list and ends behind it;
+// WARPS warps a row, each every WARPS-th part.  Latency alone, 3 to 5 us: a chain of four loads, and one more for every eight parts of a warp.
+template <typename T, int D, int ROWS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS * ROWS) paged_combine_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int LANES = 32 * WARPS;
+  __shared__ float red[ROWS][WARPS][D];
+  __shared__ float red_m[ROWS][WARPS], red_l[ROWS][WARPS];
   chain_wait();
-  const int c = blockIdx.x, sub = threadIdx.x / 128, row = blockIdx.y * COMBINE_ROWS + sub, tid = threadIdx.x % 128, warp = tid >> 5, lane = tid & 31;
+  const int c = blockIdx.x, sub = threadIdx.x / LANES, row = blockIdx.y * ROWS + sub, tid = threadIdx.x % LANES, warp = tid >> 5, lane = tid & 31;
   const int total = a.meta[0], per = a.meta[1];
   if ((int64_t)(c + 1) * per >= total) return;
   const int4 hd = a.head[c];
@@ -416,19 +417,20 @@ __global__ void __launch_bounds__(128 * COMBINE_ROWS) paged_combine_kernel(const
   const int last = (hd.y - 1) / per, pieces = ra.there ? last - c + 1 : 0;
   auto slot = [&](int p) { return 2 * (c + p) + (p == 0 && hd.x > c * per ? 1 : 0); };
   float m = -INFINITY;
-  for (int p = tid; p < pieces; p += 128) m = fmaxf(m, a.part_stat[slot(p) * ITEM_ROWS + row].x);
+  for (int p = tid; p < pieces; p += LANES) m = fmaxf(m, a.part_stat[slot(p) * ITEM_ROWS + row].x);
 #pragma unroll
   for (int s = 1; s < 32; s *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
   if (lane == 0) red_m[sub][warp] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(red_m[sub][0], red_m[sub][1]), fmaxf(red_m[sub][2], red_m[sub][3]));
+#pragma unroll
+  for (int x = 0; x < WARPS; ++x) m = fmaxf(m, red_m[sub][x]);
   // pieces p = warp, warp + 4, ...: a lane D / 32 columns
   constexpr int E = D / 32;
   float v[E], l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 8
-  for (int p = warp; p < pieces; p += 4) {
+  for (int p = warp; p < pieces; p += WARPS) {
     const float2 st = a.part_stat[slot(p) * ITEM_ROWS + row];
     const float* src = a.part + ((int64_t)slot(p) * ITEM_ROWS + row) * D + lane * E;
     float y[E];
@@ -449,9 +451,15 @@ __global__ void __launch_bounds__(128 * COMBINE_ROWS) paged_combine_kernel(const
   if (lane == 0) red_l[sub][warp] = l;
   __syncthreads();
   if (!ra.there) return;
-  l = (red_l[sub][0] + red_l[sub][1]) + (red_l[sub][2] + red_l[sub][3]);
-  const float(*r)[D] = red[sub];
-  if (tid < D) ((T*)a.o)[ra.o * D + tid] = from_f32<T>(ra.empty ? 0.f : ((r[0][tid] + r[1][tid]) + (r[2][tid] + r[3][tid])) / l);
+  l = red_l[sub][0];
+#pragma unroll
+  for (int x = 1; x < WARPS; ++x) l += red_l[sub][x];
+  if (tid < D) {
+    float y = red[sub][0][tid];
+#pragma unroll
+    for (int x = 1; x < WARPS; ++x) y += red[sub][x][tid];
+    ((T*)a.o)[ra.o * D + tid] = from_f32<T>(ra.empty ? 0.f : y / l);
+  }
   if (tid == 0) a.lse[ra.lse] = ra.empty ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
@@ -530,6 +538,21 @@ int launch_attn(const AttnArgs& a, const ha_paged_params& p, int ctas, cudaStrea
   else if (a.pack > 1) HA_PAGED_VARIANT(false, true);
   else HA_PAGED_VARIANT(false, false);
 #undef HA_PAGED_VARIANT
+  HA_LAUNCHED("ha_paged_attn");
+  return HA_OK;
+}
+
+template <int ROWS, int WARPS>
+int launch_combine(const AttnArgs& a, const ha_paged_params& p, int ctas, cudaStream_t st) {
+  const dim3 grid(ctas - 1, (std::min(attn_rows(p), ITEM_ROWS) + ROWS - 1) / ROWS);
+  auto launch = [&](auto kernel) { launch_chained(kernel, grid, 32 * WARPS * ROWS, 0, st, a); };
+  if (p.d == 64) {
+    if (p.dtype == HA_BF16) launch(paged_combine_kernel<__nv_bfloat16, 64, ROWS, WARPS>);
+    else launch(paged_combine_kernel<__half, 64, ROWS, WARPS>);
+  } else {
+    if (p.dtype == HA_BF16) launch(paged_combine_kernel<__nv_bfloat16, 128, ROWS, WARPS>);
+    else launch(paged_combine_kernel<__half, 128, ROWS, WARPS>);
+  }
   HA_LAUNCHED("ha_paged_attn");
   return HA_OK;
 }
@@ -622,15 +645,11 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
     else rc = bf ? launch_attn<__nv_bfloat16, 128>(a, p, now, st) : launch_attn<__half, 128>(a, p, now, st);
     if (rc != HA_OK) return rc;
     if (now == 1 || cluster > 0) continue;
-    const dim3 grid(now - 1, ((attn_rows(p) < ITEM_ROWS ? attn_rows(p) : ITEM_ROWS) + COMBINE_ROWS - 1) / COMBINE_ROWS);
-    if (p.d == 64) {
-      if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 64>, grid, 128 * COMBINE_ROWS, 0, st, a);
-      else launch_chained(paged_combine_kernel<__half, 64>, grid, 128 * COMBINE_ROWS, 0, st, a);
-    } else {
-      if (bf) launch_chained(paged_combine_kernel<__nv_bfloat16, 128>, grid, 128 * COMBINE_ROWS, 0, st, a);
-      else launch_chained(paged_combine_kernel<__half, 128>, grid, 128 * COMBINE_ROWS, 0, st, a);
-    }
-    HA_LAUNCHED("ha_paged_attn");
+    // many parts of an item: more warps to a row (1 x 32768 tokens, two K/V heads, 148 parts each: 16.8 us, 18.1 by four warps; 4 x 30000, 37 parts: 21.8 and 22.3); few: fewer
+    // blocks (8 x 30000, 18 parts: 28.7 us by two rows of four warps, 29.8 by eight warps a row; 32 x 8192: 27.1 and 29.2)
+    if (now >= 32 * all * attn_items(p)) rc = launch_combine<1, 8>(a, p, now, st);
+    else rc = launch_combine<2, 4>(a, p, now, st);
+    if (rc != HA_OK) return rc;
   }
   return HA_OK;
 }
