@@ -151,12 +151,12 @@ __device__ __forceinline__ uint2 quantise(const float (&x)[PART], __half2& scale
 
 // One block a token, D / 16 lanes a row, sixteen elements a lane, which keeps its cosines and sines for all the heads that it meets; two rows of a
 // lane under way at once.  Bound by the bytes of q, k and v for prompts, by the chain length -> page -> store for single tokens.  32768 tokens, 32 + 2 + 2
-// heads x 128: 108 us, 5.7 TB/s; 2 x 8191 tokens, 32 + 32 + 32 heads x 64, into 4 bits: 92 us, issue-bound by the codes' arithmetic (half of it in pairs: 95 us without); one token of 32
-// sequences: 2.3 us.  (Launch bounds for 5, 6 or 8 blocks of an SM spill or gain nothing.)
-template <typename T, int D, int BITS, bool WIDE>
-__global__ void __launch_bounds__(128) paged_append_kernel(const AppendArgs a) {
+// heads x 128: 98 us, 6.3 TB/s; 2 x 8191 tokens, 32 + 32 + 32 heads x 64, into 4 bits: 77 us, 3.7 TB/s, the codes' arithmetic beside the copies; one token of 32
+// sequences: 2.4 us.  (Launch bounds for 5, 6 or 8 blocks of an SM spill or gain nothing.)
+template <typename T, int D, int BITS, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendArgs a) {
   chain_begin();
-  constexpr int LANES = D / PART, GROUPS = 128 / LANES;
+  constexpr int LANES = D / PART, GROUPS = THREADS / LANES;
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   for (int64_t tok = blockIdx.x; tok < a.tokens; tok += gridDim.x) {
     const int b = a.by_n((int)tok), i = (int)(tok - (int64_t)b * a.n);
@@ -186,9 +186,9 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendArgs a) {
     if (!live) {                                      // padding: zeros, and nothing to keep
       const uint4 zero = make_uint4(0, 0, 0, 0);
       if (a.q)
-        for (int e = threadIdx.x; e < a.H * D / 8; e += 128) reinterpret_cast<uint4*>((T*)a.q_out + tok * a.H * D)[e] = zero;
+        for (int e = threadIdx.x; e < a.H * D / 8; e += THREADS) reinterpret_cast<uint4*>((T*)a.q_out + tok * a.H * D)[e] = zero;
       if (a.k_out)
-        for (int e = threadIdx.x; e < a.Hk * D / 8; e += 128) reinterpret_cast<uint4*>((T*)a.k_out + tok * a.Hk * D)[e] = zero;
+        for (int e = threadIdx.x; e < a.Hk * D / 8; e += THREADS) reinterpret_cast<uint4*>((T*)a.k_out + tok * a.Hk * D)[e] = zero;
       continue;
     }
     Turn turn;
@@ -357,12 +357,21 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
   }
 }
 
+template <typename T, int D, int BITS, int THREADS>
+static void launch_append_block(const AppendArgs& a, bool wide, unsigned grid, cudaStream_t st) {
+  if (wide) launch_chained(paged_append_kernel<T, D, BITS, true, THREADS>, grid, THREADS, 0, st, a);
+  else launch_chained(paged_append_kernel<T, D, BITS, false, THREADS>, grid, THREADS, 0, st, a);
+}
+// Threads of a block, which takes a token.  Fewer make more tokens resident, whose chains hide one another: 64 where there are more tokens than blocks of 128 are resident
+// (five an SM), or 32 where the query rows are few, too.  32768 tokens, 32 + 2 + 2 heads x 128: 107.7 us by 128 threads, 97.8 by 64, 102.1 by 32; 55656 tokens, 12 + 2 + 2
+// heads: 127.7, 87.8, 83.0; 2 x 8191 tokens into 4 bits, 32 + 32 + 32 heads x 64, and back: 122.9, 109.8, 107.5; 32 tokens: 2.4, 2.9, 3.8.
 template <typename T, int D, int BITS>
 static int launch_append(const AppendArgs& a, bool wide, cudaStream_t st) {
-  const int64_t most = (int64_t)sm_count() * 512;
+  const int64_t sms = sm_count(), most = sms * 512;
   const unsigned grid = (unsigned)(a.tokens < most ? a.tokens : most);
-  if (wide) launch_chained(paged_append_kernel<T, D, BITS, true>, grid, 128, 0, st, a);
-  else launch_chained(paged_append_kernel<T, D, BITS, false>, grid, 128, 0, st, a);
+  if (a.tokens <= 5 * sms) launch_append_block<T, D, BITS, 128>(a, wide, grid, st);
+  else if (a.H * (D / PART) > 128) launch_append_block<T, D, BITS, 64>(a, wide, grid, st);
+  else launch_append_block<T, D, BITS, 32>(a, wide, grid, st);
   HA_LAUNCHED("ha_paged_append");
   return HA_OK;
 }

@@ -483,6 +483,16 @@ def test_append_without_queries_and_long():
     append_case(4, BF, 64, 32, 2, 64, [3], 999, rot=64, rope_dtype=BF)
 
 
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('dtype', [BF, HF])
+@pytest.mark.parametrize('d,H,Hk', [(128, 18, 2), (128, 3, 3), (64, 34, 17), (64, 6, 2)])
+def test_append_many_tokens(bits, dtype, d, H, Hk):
+    """more tokens than are under way at once: blocks of fewer threads; padding among them, rows off their boundaries, none to rotate"""
+    append_case(bits, dtype, d, H, Hk, 48, [5, 0], 420, counts=[401, 17], rot=d // 2)
+    append_case(bits, dtype, d, H, Hk, 16, [1], 760, rot=d, rope_dtype=dtype, order='odd')
+    append_case(bits, dtype, d, H, Hk, 100, [0, 3, 9], 300, order='tokens', with_q=False)
+
+
 def test_append_empty_calls():
     cache = ha.PagedCache.allocate(2, 16, 2, 64)
     z = lambda *s: torch.zeros(*s, dtype=BF, device='cuda')
