@@ -28,6 +28,8 @@ namespace ha {
 namespace {
 
 constexpr int THREADS = 160;
+constexpr int BOX_ROWS = 32;          // rows of a tensor copy, at most: what is fetched behind the last key is less than that (49 x up to 7 tokens, 64 heads, pages of 256: 22.2 us by 64, 20.6 by 32;
+                                      // long rows alike; by 16, 1 x 131072 with 32 heads x 64 gains 2 %, 16 x 4096 by clusters loses 10 %)
 constexpr int CLUSTER_TILES = 10;     // tiles of a CTA, at most, where clusters share items
 
 template <int D>
@@ -510,7 +512,7 @@ int64_t attn_lines(const ha_paged_params& p) {
 // Tensor maps of K and V pages: boxes of as many rows as both a page and a tile are made of.
 bool attn_maps(const ha_paged_params& p, CUtensorMap* maps) {
   if (p.pages == 0) return true;
-  const int run = std::gcd(p.page_size, Stage<64>::TK);
+  const int run = std::gcd(p.page_size, BOX_ROWS);
   const int64_t row = p.page_size == 1 ? p.d : p.page_st;
   return encode_tile_map(&maps[0], p.dtype, p.k_pages, p.d, p.page_size, p.Hk, p.pages, row, p.page_sh, p.page_sp, run) &&
          encode_tile_map(&maps[1], p.dtype, p.v_pages, p.d, p.page_size, p.Hk, p.pages, row, p.page_sh, p.page_sp, run);
@@ -626,7 +628,7 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   a.part_stat = (float2*)(ws + 256 + (int64_t)ctas * 16);
   a.part = (float*)(ws + 256 + (int64_t)ctas * (16 + 2 * ITEM_ROWS * 8));
   if (p.bits == 16) {
-    while ((1 << a.run_log2) < std::gcd(p.page_size, attn_tile(p))) ++a.run_log2;
+    while ((1 << a.run_log2) < std::gcd(p.page_size, BOX_ROWS)) ++a.run_log2;
   } else {
     const int part = attn_tile(p) / 4, sc = p.d / PAGED_GROUP * 4;
     a.whole_runs = p.page_size % part == 0 && a.c.st == p.d / 2 && a.c.sst == sc &&
