@@ -630,9 +630,10 @@ int ha_paged_attn(const ha_paged_params* pp, void* stream) {
   if (p.bits == 16) {
     while ((1 << a.run_log2) < std::gcd(p.page_size, BOX_ROWS)) ++a.run_log2;
   } else {
-    const int part = attn_tile(p) / 4, sc = p.d / PAGED_GROUP * 4;
-    a.whole_runs = p.page_size % part == 0 && a.c.st == p.d / 2 && a.c.sst == sc &&
+    const int part = attn_tile(p) / 4, run = 1024 / p.d, sc = p.d / PAGED_GROUP * 4;
+    const bool together = a.c.st == p.d / 2 && a.c.sst == sc &&
                    ((uintptr_t)p.k_scales | (uintptr_t)p.v_scales | (uintptr_t)a.c.ssp | (uintptr_t)a.c.ssh) % 16 == 0;
+    a.runs = !together ? 0 : p.page_size % part == 0 ? 2 : p.page_size % run == 0 ? 1 : 0;
   }
   const cudaStream_t st = (cudaStream_t)stream;
   const bool bf = p.dtype == HA_BF16;

@@ -24,7 +24,7 @@ struct AttnArgs {
   int32_t line0, lines;               // (sequence, pack) pairs of this launch
   int32_t cluster;                    // CTAs that share an item, a cluster of them; 0: the list of tiles
   int32_t run_log2;                   // rows that are fetched together: 2^run_log2, the largest power of two that pages and tiles are made of
-  int32_t whole_runs;                 // 4 bits: a warp's keys of a tile lie together, and their scales, on 16-byte boundaries
+  int32_t runs;                       // 4 bits, rows of a page and their scales one behind the other, on 16-byte boundaries: 2 where a page holds a warp's keys of a tile, 1: a copy's
   FastDiv by_packs, by_blocks, by_group;
   float scale_log2;                   // magnitude of the softmax scale, times log2 e
   uint32_t flip;                      // sign bits of a pair of queries, where the scale is negative

@@ -28,6 +28,7 @@ struct Stage4 {
   static constexpr int NB = 2;                              // sixteens of keys that a warp takes at once
   static constexpr int KW = 16 * NB, TK = attn4_tile(D), WK = TK / 4;      // those keys; keys of a tile, a warp's of them
   static constexpr int ROW = D / 2, G = D / PAGED_GROUP, SC = 4 * G, ROWS = 8 * NQ;        // bytes of a row, of its scales; queries
+  static constexpr int RUN = 512 / ROW;                      // rows of a copy of the warp
   static constexpr int V = WK * ROW, KS = 2 * WK * ROW, VS = KS + WK * SC, BYTES = VS + WK * SC;       // a warp's stage
   // (16 rows x 128: 170 registers a thread; for a fourth CTA sums would be spilled, 80 -> 107 us at 64 x 32768 tokens.  8 rows gain by it: 59.0 -> 57.1)
   static constexpr int CTAS = D == 128 && NQ == 2 ? 3 : 4, NS = 2;
@@ -37,7 +38,7 @@ struct Stage4 {
   static constexpr int SMEM = 4 * WARP + PARTS + 4 * ITEM_ROWS * 8 + (2 * MAX_LINES + 8) * 4 + 32 + MAX_LINES;
   static constexpr int ROUNDS = NQ;                          // in which the warps' sums are joined: column ranges that fit a stage
   static_assert(ROWS * D / ROUNDS * 4 <= BYTES, "a warp's sums fit a stage");
-  static_assert(WK * ROW == 2048 && WK * SC == 256 && WARP % 16 == 0, "copies of a warp's rows and scales");
+  static_assert(WK * ROW == 2048 && WK * SC == 256 && RUN * SC == 64 && WARP % 16 == 0, "copies of a warp's rows and scales");
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
@@ -485,7 +486,7 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
     const Place f = *place;
     const int key0 = f.tile * TK + warp * WK, left = f.keys - key0;
     const uint32_t dst = base + s * S::BYTES;
-    if (a.whole_runs) {
+    if (a.runs == 2) {
       // rows that lie together, and their scales (of all WK, whatever they are behind the last key: the page has them)
       if (left > 0) {
         const int col = a.c.by_page(key0), slot = key0 - col * a.c.page_size, page = f.table[col];
@@ -500,6 +501,28 @@ __global__ void __launch_bounds__(128, (Stage4<D, NQ>::CTAS)) paged_attn4_kernel
           cp_async16(dst + S::KS + lane * 16, sc, 16);
         }
       }
+    } else if (a.runs == 1) {
+      // ... in runs of RUN, one a copy of the warp; scales by the lanes that look the run up (64 x 32768 tokens, pages of 16: 97 us row by row, 86 so, 81 where pages hold the
+      // whole part; 1 x 262144, 32 heads x 64, pages of 32: 179, 149, 137)
+      constexpr int RUN = S::RUN;
+      const int first_row = RUN * ((lane & 15) >> 2);
+      int64_t off = -1, off_s = 0;
+      if (first_row < left) {
+        const int col = a.c.by_page(key0 + first_row), slot = key0 + first_row - col * a.c.page_size, page = f.table[col];
+        if (paged_checked(a.c, page)) {
+          off = page * a.c.sp + f.head + (int64_t)slot * S::ROW;
+          off_s = page * a.c.ssp + f.head_s + (int64_t)slot * S::SC;
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int64_t from = __shfl_sync(0xffffffffu, off, 4 * y);
+        if (from >= 0) {
+          cp_async16(dst + lane * 16 + 512 * y, a.c.k + from + lane * 16, 16);
+          cp_async16(dst + lane * 16 + S::V + 512 * y, a.c.v + from + lane * 16, 16);
+        }
+      }
+      if (off >= 0) cp_async16(dst + S::KS + lane * 16, (lane < 16 ? a.c.ks : a.c.vs) + off_s + (lane & 3) * 16, 16);
     } else {
       constexpr int C = S::ROW / 16;
       for (int e = lane; e < WK * C; e += 32) {
