@@ -111,14 +111,15 @@ inline int sm_count() {
 
 // Opt-in dynamic shared memory size of a kernel: a per-device function attribute, set at the first launch on each device
 // (one process may drive several GPUs) instead of before every launch.
-#define HA_SMEM_ATTR_ONCE(kernel, bytes, where)                                                        \
+#define HA_SMEM_ATTR_ONCE(kernel, bytes, where) HA_ATTR_ONCE(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes, where)
+#define HA_ATTR_ONCE(kernel, attribute, value, where)                                                  \
   do {                                                                                                 \
     static std::atomic<unsigned long long> _done{0};                                                   \
     int _dev = 0;                                                                                      \
     cudaGetDevice(&_dev);                                                                              \
     const unsigned long long _bit = 1ull << (_dev & 63);                                               \
     if (!(_done.load(std::memory_order_acquire) & _bit)) {                                             \
-      HA_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), where); \
+      HA_CUDA_OK(cudaFuncSetAttribute(kernel, attribute, value), where);                               \
       _done.fetch_or(_bit, std::memory_order_release);                                                 \
     }                                                                                                  \
   } while (0)

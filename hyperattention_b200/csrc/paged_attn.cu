@@ -31,6 +31,7 @@ constexpr int THREADS = 160;
 constexpr int BOX_ROWS = 32;          // rows of a tensor copy, at most: what is fetched behind the last key is less than that (49 x up to 7 tokens, 64 heads, pages of 256: 22.2 us by 64, 20.6 by 32;
                                       // long rows alike; by 16, 1 x 131072 with 32 heads x 64 gains 2 %, 16 x 4096 by clusters loses 10 %)
 constexpr int CLUSTER_TILES = 10;     // tiles of a CTA, at most, where clusters share items
+constexpr int CLUSTER_TILES_16 = 6;   // ... in clusters of 16
 
 template <int D>
 struct Stage {
@@ -491,13 +492,17 @@ int attn_ctas(const ha_paged_params& p, int lines) {
 // second launch (1 x 515 tokens, two K/V heads: 8.2 -> 6.9 us on the device, 7.1 -> 2.7 us for the call).  Every item gets the same CTAs, however long it is, so that
 // the list of tiles, which deals them out evenly, is for what takes longer than the joining: with CLUSTER_TILES 7 a batch of 16 x 4096 goes by the list, 17.4 us for 15.3 (1 x 5000 gains:
 // 12.1 for 13.6); with 20, 1 x 8000 by clusters of 8, 19.5 us for 12.5; with 40 a batch of 32 x 8192, 37 us for 28.
+// Clusters of 16 (more than every GPU promises, but all of these) where they take no more than half of the room, since they need theirs within a part of the GPU: 1 x 515
+// 7.05 -> 6.5 us, 1 x 5000 13.8 -> 10.0, 1 x 2051 in 4 bits 10.2 -> 9.2, 1 x 8000 in 4 bits 16.7 -> 12.2 (with all of the room 8 x 1000 took 13.7 us, by clusters of 8 7.7).  At
+// eight tiles a CTA the list is faster again: 1 x 8000 12.5 and 12.1 us, 1 x 16000 in 4 bits 17.2 and 15.6.
 int attn_cluster(const ha_paged_params& p) {
   const int64_t units = p.B * attn_packs(p) * attn_items(p);
   const int64_t tiles = ((int64_t)p.columns * p.page_size + attn_tile(p) - 1) / attn_tile(p), resident = (int64_t)sm_count() * attn_resident(p);
   if (units > resident || tiles == 0) return 0;
   int c = 1;
   while (c < 8 && c < tiles && units * 2 * c <= resident) c *= 2;
-  return (tiles + c - 1) / c <= CLUSTER_TILES ? c : 0;
+  if (c == 8 && tiles > 8 && units * 32 <= resident) c = 16;
+  return (tiles + c - 1) / c <= (c == 16 ? CLUSTER_TILES_16 : CLUSTER_TILES) ? c : 0;
 }
 
 // Lines of one launch: no more than shared memory counts, their tiles within 31 bits.
@@ -533,6 +538,7 @@ int launch_attn(const AttnArgs& a, const ha_paged_params& p, int ctas, cudaStrea
 #define HA_PAGED_VARIANT(cluster, packed)                                                          \
   do {                                                                                             \
     HA_SMEM_ATTR_ONCE((paged_attn_kernel<T, D, cluster, packed>), S::SMEM, "ha_paged_attn");       \
+    if (cluster) HA_ATTR_ONCE((paged_attn_kernel<T, D, cluster, packed>), cudaFuncAttributeNonPortableClusterSizeAllowed, 1, "ha_paged_attn"); \
     launch(paged_attn_kernel<T, D, cluster, packed>);                                              \
   } while (0)
   if (a.cluster > 0 && a.pack > 1) HA_PAGED_VARIANT(true, true);

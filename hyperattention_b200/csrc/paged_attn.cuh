@@ -327,9 +327,8 @@ __device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
 
 // End of an item that a cluster shares: each CTA joins its share of the rows from all CTAs' parts, read over distributed shared memory.  The first four warps of every
 // CTA call it, those of a CTA without keys, too (a negative denominator); no CTA leaves before the others have read its part.
-template <typename T, int D, bool PACKED>
-__device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* sums, const float2* stat, int line, int item, int keys, int last) {
-  cluster_sync();
+template <typename T, int D, bool PACKED, int MOST>
+__device__ __forceinline__ void cluster_join(const AttnArgs& a, const float* sums, const float2* stat, int line, int item, int keys, int last) {
   const int tid = threadIdx.x, rank = blockIdx.x % a.cluster;
   constexpr int LANES = D / 4;                 // threads of a row, four columns each
   for (int row = rank + a.cluster * (tid / LANES); row < min(a.pack * a.group, ITEM_ROWS); row += a.cluster * (128 / LANES)) {
@@ -337,20 +336,20 @@ __device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* s
     if (!ra.there) continue;
     const int col = tid % LANES * 4;
     float m = -INFINITY, l = 0.f;
-    float2 st[8];
-    float4 f[8];
+    float2 st[MOST];
+    float4 f[MOST];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < MOST; ++x) {
       st[x] = make_float2(-INFINITY, -1.f);
       if (x >= a.cluster) continue;
       asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(st[x].x), "=f"(st[x].y) : "r"(cluster_at(stat + row, x)));
       asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[x].x), "=f"(f[x].y), "=f"(f[x].z), "=f"(f[x].w) : "r"(cluster_at(sums + row * D + col, x)));
     }
 #pragma unroll
-    for (int x = 0; x < 8; ++x) m = fmaxf(m, st[x].x);
+    for (int x = 0; x < MOST; ++x) m = fmaxf(m, st[x].x);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < MOST; ++x) {
       if (st[x].y < 0.f) continue;
       const float w = st[x].x == -INFINITY ? 0.f : fast_exp2(st[x].x - m);
       l = fmaf(w, st[x].y, l);
@@ -363,6 +362,12 @@ __device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* s
     *reinterpret_cast<uint2*>((T*)a.o + ra.o * D + col) = ra.empty ? make_uint2(0, 0) : make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
     if (col == 0) a.lse[ra.lse] = ra.empty ? -INFINITY : (m + log2f(l)) * LN2;
   }
+}
+template <typename T, int D, bool PACKED>
+__device__ __forceinline__ void cluster_finish(const AttnArgs& a, const float* sums, const float2* stat, int line, int item, int keys, int last) {
+  cluster_sync();
+  if (a.cluster > 8) cluster_join<T, D, PACKED, 16>(a, sums, stat, line, item, keys, last);
+  else cluster_join<T, D, PACKED, 8>(a, sums, stat, line, item, keys, last);
   cluster_sync();
 }
 

@@ -634,6 +634,7 @@ int launch4(const AttnArgs& a, int ctas, cudaStream_t st) {
 #define HA_PAGED_VARIANT(cluster, packed)                                                          \
   do {                                                                                             \
     HA_SMEM_ATTR_ONCE((paged_attn4_kernel<T, D, NQ, cluster, packed>), S::SMEM, "ha_paged_attn");  \
+    if (cluster) HA_ATTR_ONCE((paged_attn4_kernel<T, D, NQ, cluster, packed>), cudaFuncAttributeNonPortableClusterSizeAllowed, 1, "ha_paged_attn"); \
     launch(paged_attn4_kernel<T, D, NQ, cluster, packed>);                                         \
   } while (0)
   if (a.cluster > 0 && a.pack > 1) HA_PAGED_VARIANT(true, true);
