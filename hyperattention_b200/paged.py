@@ -129,17 +129,22 @@ class PagedCache:
         return tuple(out)
 
 
-def _call(name, cache, *args):
+_transforms = torch._C._are_functorch_transforms_active
+
+
+def _handle(cache):
     # forward-mode differentiation and function transforms would lose their tangents without a word
-    assert forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active(), \
-        'the operators of the paged cache have no gradient: call them under torch.no_grad()'
-    r = getattr(_EXT or _ext(), name)(cache._handle or cache._open(), *args)
-    if r.__class__ is int:
-        L.check(r, 'ha_paged_' + name)
-    if r is NotImplemented:              # an earlier launch has reported a failure: raised here, as at every call into the library
+    assert forward_ad._current_level < 0 and not _transforms(), 'the operators of the paged cache have no gradient: call them under torch.no_grad()'
+    return cache._handle or cache._open()
+
+
+def _settle(r, name, cache):
+    """What an operator's host side answers in the place of outputs: a status, or NotImplemented where an earlier launch has reported a failure, which is raised
+    here, as at every call into the library (and gone when it has been raised elsewhere meanwhile)."""
+    if r is NotImplemented:
         ops._raise_if_failed(*ops._status_words(cache.device))
-        return _call(name, cache, *args)
-    return r
+    else:
+        L.check(r, 'ha_paged_' + name)
 
 
 def paged_append(cache, k, v, table, lengths, counts=None, rope=None, q=None, return_keys=False):
@@ -153,7 +158,11 @@ def paged_append(cache, k, v, table, lengths, counts=None, rope=None, q=None, re
 
     Returns the rotated queries [B, n, heads, head_dim] (None without q); with return_keys, (queries, rotated keys [B, n, kv_heads, head_dim]): what the
     prompt's own attention takes.  Padding rows of both are zero.  Two rows of one call must not go to the same slot."""
-    return _call('append', cache, k, v, table, lengths, counts, rope, q, return_keys)
+    r = (_EXT or _ext()).append(_handle(cache), k, v, table, lengths, counts, rope, q, return_keys)
+    if r.__class__ is int or r is NotImplemented:
+        _settle(r, 'append', cache)
+        return paged_append(cache, k, v, table, lengths, counts, rope, q, return_keys)
+    return r
 
 
 def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
@@ -166,10 +175,18 @@ def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
     query heads share a K/V head.  Keys are read once for 16 query rows of a K/V head, those of neighbouring tokens where a token has fewer, and again
     for the next 16: made for one to a few tokens a sequence; prompts belong to HyperAttention or flash_attn_func.  Over a cache in 4 bits,
     queries of 1e34 and more are not told from infinite ones."""
-    return _call('attn', cache, q, table, lengths, counts, float(softmax_scale or cache.head_dim ** -0.5))
+    r = (_EXT or _ext()).attn(_handle(cache), q, table, lengths, counts, float(softmax_scale or cache.head_dim ** -0.5))
+    if r.__class__ is int or r is NotImplemented:
+        _settle(r, 'attn', cache)
+        return paged_attn_func(q, cache, table, lengths, counts, softmax_scale)
+    return r
 
 
 def paged_gather(cache, table, lengths, rows):
     """Positions 0 .. rows - 1 of every sequence as dense (k, v) [B, kv_heads, rows, head_dim] in the cache's type, zero from lengths[b] (int32 [B]) on: the
     layout that HyperAttention takes."""
-    return _call('gather', cache, table, lengths, int(rows))
+    r = (_EXT or _ext()).gather(_handle(cache), table, lengths, int(rows))
+    if r.__class__ is int or r is NotImplemented:
+        _settle(r, 'gather', cache)
+        return paged_gather(cache, table, lengths, rows)
+    return r
