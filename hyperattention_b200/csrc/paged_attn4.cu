@@ -1,8 +1,10 @@
 // Attention over 4-bit pages (the scheme of paged_attn.cu: items, list of tiles, parts).
 //
 // A quarter of the bytes, so that the work on a value counts: at the memory's rate an SM has some three instructions a value.  Codes become operands without
-// arithmetic: code * 2^-24 and code * 2^-20 are fp16 numbers (subnormal ones) whose bits are the code's own, so that one mask makes a
-// pair; steps and offsets are applied to the products.  With s, m of a group (a row's 64 elements):
+// arithmetic: code * 2^-24, 2^-22, 2^-20 and 2^-18 are fp16 numbers (subnormal ones) whose bits are the code's own, so that one mask makes a
+// pair; steps and offsets are applied to the products.  Tensor cores cut products off as if a subnormal factor were as large as 2^-14: K's codes of the
+// words shifted by six stand higher up and lose less, and those of one place go into one product (score of one key, fp16 queries: error 2.3e-6
+// with the places 2^-24 and 2^-20 side by side, 1.2e-6 so; bf16: 9e-7 and 5e-7.  V's products have the weights' rounding above that).  With s, m of a group (a row's 64 elements):
 //   q . k = sum over groups of s (q . code) + m sum(q),      o = sum p (s code + m) = sum (p s) (code - 7.5) + sum p (m + 7.5 s)
 // Both products are taken transposed, keys (and then V's elements) as the 16 rows and queries as the 8 columns of mma.sync.m16n8k16: eight query heads
 // cost half of what sixteen do, in products and in everything done per score.
@@ -84,7 +86,7 @@ struct Worker4 {
   int lane;
 
   // Query operands: fp16, every query times the power of two that brings its largest element to 2^13 .. 2^14.  Lane c of a query's four holds elements
-  // 16 c .. 16 c + 15 of each group, paired as the codes come out of their words: (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
+  // 16 c .. 16 c + 15 of each group, paired as the codes come out of their words: (0, 4), (1, 5) / 16, (2, 6) / 4, (3, 7) / 64.
   __device__ __forceinline__ void begin(const AttnArgs& a, int line, int item) {
     const int c = lane & 3;
     const uint8_t* q = query_of(a, line, item);
@@ -127,13 +129,11 @@ struct Worker4 {
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int y = 0; y < 4; ++y) {
+          const float by = up * (y == 0 ? 1.f : y == 1 ? 0x1p-4f : y == 2 ? 0x1p-2f : 0x1p-6f);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float* e8 = &x[g][8 * u + 2 * h];
-            f[(g * 2 + u) * 2 + h][2 * n] = pack2<__half>(e8[0] * up, e8[4] * up);
-            f[(g * 2 + u) * 2 + h][2 * n + 1] = pack2<__half>(e8[1] * up * 0.0625f, e8[5] * up * 0.0625f);
-          }
+          for (int u = 0; u < 2; ++u) f[g * 4 + y][2 * n + u] = pack2<__half>(x[g][8 * u + y] * by, x[g][8 * u + y + 4] * by);
+        }
       ref[n][0] = ref[n][1] = -INFINITY;
       below[n] = 0;
       sum[n] = 0;
@@ -237,22 +237,20 @@ struct Worker4 {
 #pragma unroll
           for (int e = 0; e < 4; ++e) d[g][n][e] = 0.f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int y = 0; y < 4; ++y)             // elements y, y + 4 of the words
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const uint32_t a = w[0][u * G + g] >> (8 * h), b = w[1][u * G + g] >> (8 * h);
-            const uint32_t k[4] = {a & M0, b & M0, a & M1, b & M1};
-            const int step = (g * 2 + u) * 2 + h;
-            if constexpr (NQ == 1) {
-              mma16816<__half>(d[g][0], k, qf[step][0], qf[step][1]);
-            } else {
-              const uint4 q = qs[step * 32 + lane];
-              mma16816<__half>(d[g][0], k, q.x, q.y);
-              mma16816<__half>(d[g][1], k, q.z, q.w);
-            }
+        for (int g = 0; g < G; ++g) {
+          constexpr uint32_t M[4] = {0x000f000fu, 0x00f000f0u, 0x003c003cu, 0x03c003c0u};
+          const int by = y < 2 ? 0 : 6, step = g * 4 + y;
+          const uint32_t k[4] = {(w[0][g] >> by) & M[y], (w[1][g] >> by) & M[y], (w[0][G + g] >> by) & M[y], (w[1][G + g] >> by) & M[y]};
+          if constexpr (NQ == 1) {
+            mma16816<__half>(d[g][0], k, qf[step][0], qf[step][1]);
+          } else {
+            const uint4 q = qs[step * 32 + lane];
+            mma16816<__half>(d[g][0], k, q.x, q.y);
+            mma16816<__half>(d[g][1], k, q.z, q.w);
           }
+        }
       uint64_t unit[NQ], qsum[G][NQ];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
