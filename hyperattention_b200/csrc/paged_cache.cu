@@ -152,9 +152,10 @@ __device__ __forceinline__ uint2 quantise(const float (&x)[PART], __half2& scale
 // One block a token, D / 16 lanes a row, sixteen elements a lane, which keeps its cosines and sines for all the heads that it meets; two rows of a
 // lane under way at once.  Bound by the bytes of q, k and v for prompts, by the chain length -> page -> store for single tokens.  32768 tokens, 32 + 2 + 2
 // heads x 128: 98 us, 6.3 TB/s; 2 x 8191 tokens, 32 + 32 + 32 heads x 64, into 4 bits: 77 us, 3.7 TB/s, the codes' arithmetic beside the copies; one token of 32
-// sequences: 2.4 us.  (Launch bounds for 5, 6 or 8 blocks of an SM spill or gain nothing.)
+// sequences: 2.4 us.  (16 bits: 20 warps an SM, 102 registers: 24 x 2319 tokens, 12 + 2 + 2 heads x 128, 82.8 -> 75.3 us; 24 warps spill.  4 bits: 16
+// warps, 128 registers: by 18 or 20 with spilled ones 107 -> 114 us, by fewer with more 124.)
 template <typename T, int D, int BITS, bool WIDE, int THREADS>
-__global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(THREADS, (BITS == 16 ? 640 : 512) / THREADS) paged_append_kernel(const AppendArgs a) {
   chain_begin();
   constexpr int LANES = D / PART, GROUPS = THREADS / LANES;
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
@@ -364,7 +365,7 @@ static void launch_append_block(const AppendArgs& a, bool wide, unsigned grid, c
 }
 // Threads of a block, which takes a token.  Fewer make more tokens resident, whose chains hide one another: 64 where there are more tokens than blocks of 128 are resident
 // (five an SM), or 32 where the query rows are few, too.  32768 tokens, 32 + 2 + 2 heads x 128: 107.7 us by 128 threads, 97.8 by 64, 102.1 by 32; 55656 tokens, 12 + 2 + 2
-// heads: 127.7, 87.8, 83.0; 2 x 8191 tokens into 4 bits, 32 + 32 + 32 heads x 64, and back: 122.9, 109.8, 107.5; 32 tokens: 2.4, 2.9, 3.8.
+// heads: 127.7, 87.8, 75.3; 2 x 8191 tokens into 4 bits, 32 + 32 + 32 heads x 64, and back: 122.9, 109.8, 107.5; 32 tokens: 2.4, 2.9, 3.8.
 template <typename T, int D, int BITS>
 static int launch_append(const AppendArgs& a, bool wide, cudaStream_t st) {
   const int64_t sms = sm_count(), most = sms * 512;
