@@ -314,9 +314,15 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids, new_tokens, counts=None, cache=None, page_size=64, bits=16, graph=True):
-        """The most probable new_tokens tokens behind a prompt, one by one: int64 [b, new_tokens].  counts: int32 [b] prompt lengths where input_ids are padded
-        on the right.  cache: an empty DecoderCache to use; made for the call otherwise.  graph: the steps behind the second token replay a CUDA graph."""
+        """The most probable new_tokens tokens behind a prompt, one by one: int64 [b, new_tokens].  counts: int32 [b] prompt lengths, 1 .. sq, where input_ids are
+        padded on the right (their values are read on the host).  cache: an empty DecoderCache to use; made for the call otherwise.  graph: the steps behind the second token replay a CUDA graph."""
         b, sq = input_ids.shape
+        assert sq >= 1, 'a prompt has a token at least'
+        if counts is not None:
+            assert counts.shape == (b,) and counts.dtype == torch.int32, 'counts must be int32 [batch]'
+            # (not under a capture, where nothing can be read: the index below stays within the prompt all the same)
+            if not (counts.is_cuda and torch.cuda.is_current_stream_capturing()):
+                assert all(1 <= c <= sq for c in counts.tolist()), 'counts must be between 1 and the length of the padded prompts'
         w = self.transformer.output_layer.weight
         if cache is None:
             cache = DecoderCache(self.config, b, sq + new_tokens, page_size, bits, w.dtype, w.device)
@@ -325,7 +331,7 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
         if new_tokens == 0:
             return out
         logits = self(input_ids, cache, counts)
-        last = logits[:, -1] if counts is None else logits[torch.arange(b, device=logits.device), counts.long() - 1]
+        last = logits[:, -1] if counts is None else logits[torch.arange(b, device=logits.device), counts.long().clamp(1, sq) - 1]
         ids = last.argmax(-1, keepdim=True)
         out[:, :1] = ids
         replay = None

@@ -1,0 +1,29 @@
+"""Generation without a GPU: what is refused before the prompt runs (past the checks, the cache's operators themselves refuse CPU tensors, by another message)."""
+import pytest
+import torch
+
+from hyperattention_b200.llm import ChatGLM2ShapedDecoder, chatglm2_config
+
+
+@pytest.fixture(scope='module')
+def model():
+    cfg = chatglm2_config(num_layers=2, hidden_size=64, num_attention_heads=2, kv_channels=64, ffn_hidden_size=64, padded_vocab_size=50)
+    return ChatGLM2ShapedDecoder(cfg, seed=1, dtype=torch.bfloat16).eval()
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+@pytest.mark.parametrize('counts', [_i32(7, 0), _i32(-1, 7), _i32(8, 3), _i32(7), _i32(7, 3, 1), torch.tensor([7, 3]), _i32(7, 3)[:, None]],
+                         ids=['none', 'negative', 'beyond the prompt', 'too few', 'too many', 'int64', 'two dimensions'])
+@pytest.mark.parametrize('graph', [True, False])
+def test_generate_refuses_counts(model, counts, graph):
+    """a sequence without tokens has no last position; one behind the prompt's end would index logits that are not there"""
+    with pytest.raises(AssertionError, match='counts'):
+        model.generate(torch.zeros(2, 7, dtype=torch.int64), 3, counts=counts, graph=graph)
+
+
+def test_generate_refuses_an_empty_prompt(model):
+    with pytest.raises(AssertionError, match='prompt'):
+        model.generate(torch.zeros(2, 0, dtype=torch.int64), 3)
