@@ -178,6 +178,11 @@ class DecoderCache:
         ang = torch.outer(torch.arange(self.capacity, device=device, dtype=torch.float64), inv)
         self.rope = torch.stack([ang.cos(), ang.sin()], -1).float()
 
+    def check(self, config, batch, more):
+        """Refuses what the cache is not for: `batch` sequences of a model, `more` tokens behind those that it holds."""
+        assert batch == self.batch and len(self.layers) == config.num_layers, 'the cache is for another batch or model'
+        assert self.length + more <= self.capacity, f'the cache holds {self.capacity} tokens a sequence'
+
     def clear(self):
         self.length = 0
         self.held.zero_()
@@ -293,8 +298,7 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
         b, sq = input_ids.shape
         if cache is None:
             return self._run(input_ids, None)
-        assert b == cache.batch and len(cache.layers) == self.config.num_layers, 'the cache is for another batch or model'
-        assert cache.length + sq <= cache.capacity, f'the cache holds {cache.capacity} tokens a sequence'
+        cache.check(self.config, b, sq)
         prompt = cache.length == 0
         cache.length += sq
         return self._run(input_ids, _Step(cache, sq, counts, prompt))
@@ -315,7 +319,8 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
     @torch.no_grad()
     def generate(self, input_ids, new_tokens, counts=None, cache=None, page_size=64, bits=16, graph=True):
         """The most probable new_tokens tokens behind a prompt, one by one: int64 [b, new_tokens].  counts: int32 [b] prompt lengths, 1 .. sq, where input_ids are
-        padded on the right (their values are read on the host).  cache: an empty DecoderCache to use; made for the call otherwise.  graph: the steps behind the second token replay a CUDA graph."""
+        padded on the right (their values are read on the host).  cache: an empty DecoderCache to use, with room for the prompt and
+        all new tokens but the last; made for the call otherwise.  graph: the steps behind the second token replay a CUDA graph."""
         b, sq = input_ids.shape
         assert sq >= 1, 'a prompt has a token at least'
         if counts is not None:
@@ -327,6 +332,7 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
         if cache is None:
             cache = DecoderCache(self.config, b, sq + new_tokens, page_size, bits, w.dtype, w.device)
         assert cache.length == 0, 'the cache is not empty'
+        cache.check(self.config, b, sq + max(new_tokens - 1, 0))                 # (replayed steps do not pass forward's own check)
         out = torch.empty(b, new_tokens, dtype=torch.int64, device=input_ids.device)
         if new_tokens == 0:
             return out

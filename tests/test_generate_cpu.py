@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from hyperattention_b200.llm import ChatGLM2ShapedDecoder, chatglm2_config
+from hyperattention_b200.llm import ChatGLM2ShapedDecoder, DecoderCache, chatglm2_config
 
 
 @pytest.fixture(scope='module')
@@ -27,3 +27,23 @@ def test_generate_refuses_counts(model, counts, graph):
 def test_generate_refuses_an_empty_prompt(model):
     with pytest.raises(AssertionError, match='prompt'):
         model.generate(torch.zeros(2, 0, dtype=torch.int64), 3)
+
+
+@pytest.mark.parametrize('graph', [True, False])
+@pytest.mark.parametrize('sq,new', [(7, 11), (12, 6), (17, 1), (1, 400)])
+def test_generate_refuses_a_cache_that_is_too_small(model, graph, sq, new):
+    """16 places: the prompt and all new tokens but the last must fit, whatever runs the steps; what does not fit is refused before anything is written"""
+    cache = DecoderCache(model.config, 2, 16, page_size=8, device='cpu')
+    with pytest.raises(AssertionError, match='the cache holds 16 tokens'):
+        model.generate(torch.zeros(2, sq, dtype=torch.int64), new, cache=cache, graph=graph)
+    assert cache.length == 0 and not cache.held.any()
+    for sq, new in ((7, 10), (16, 1), (1, 16)):              # just enough: on to the operators
+        with pytest.raises(AssertionError, match='CUDA'):
+            model.generate(torch.zeros(2, sq, dtype=torch.int64), new, cache=cache, graph=graph)
+        cache.clear()
+
+
+def test_generate_refuses_the_cache_of_another_batch(model):
+    cache = DecoderCache(model.config, 3, 16, page_size=8, device='cpu')
+    with pytest.raises(AssertionError, match='another batch'):
+        model.generate(torch.zeros(2, 20, dtype=torch.int64), 3, cache=cache)
