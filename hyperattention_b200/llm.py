@@ -19,6 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from .module import HyperAttention
+from .ops import check_device_status
 from .paged import PagedCache, paged_append, paged_attn_func
 
 NUM_TOTAL_LAYERS = {
@@ -320,7 +321,8 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
     def generate(self, input_ids, new_tokens, counts=None, cache=None, page_size=64, bits=16, graph=True):
         """The most probable new_tokens tokens behind a prompt, one by one: int64 [b, new_tokens].  counts: int32 [b] prompt lengths, 1 .. sq, where input_ids are
         padded on the right (their values are read on the host).  cache: an empty DecoderCache to use, with room for the prompt and
-        all new tokens but the last; made for the call otherwise.  graph: the steps behind the second token replay a CUDA graph."""
+        all new tokens but the last; made for the call otherwise.  graph: the steps behind the second token replay a CUDA graph.  The tokens are there when
+        it returns; what a kernel reported (a table that names no page) is raised."""
         b, sq = input_ids.shape
         assert sq >= 1, 'a prompt has a token at least'
         if counts is not None:
@@ -353,4 +355,6 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
                     with torch.cuda.graph(replay):
                         ids.copy_(self._run(ids, _Step(cache, 1, None, False))[:, -1].argmax(-1, keepdim=True))
             out[:, i:i + 1] = ids
+        if not torch.cuda.is_current_stream_capturing():
+            check_device_status(w.device)                    # (a replay does not look at the status words)
         return out
