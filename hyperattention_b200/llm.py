@@ -194,7 +194,8 @@ class _Step:
 
     def __init__(self, cache, n, counts, prompt):
         self.cache, self.counts, self.prompt = cache, counts, prompt
-        self.total = cache.held + (n if counts is None else counts)
+        # (counts as the operators take them: what is written is what the cache holds)
+        self.total = cache.held + (n if counts is None else counts.clamp(0, n))
 
 
 class SelfAttention(torch.nn.Module):

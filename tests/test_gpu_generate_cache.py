@@ -1,4 +1,4 @@
-"""Generation into a caller's cache: room that is just enough, tables that name no page."""
+"""Generation into a caller's cache: room that is just enough, tables that name no page, counts out of range."""
 import pytest
 import torch
 
@@ -48,3 +48,16 @@ def test_a_table_that_names_no_page(model, graph, new):
     cache.clear()
     cache.table[0] = torch.tensor([3, 1, 0, 2], dtype=torch.int32)
     assert torch.equal(model.generate(ids, new, cache=cache, graph=graph), model.generate(ids, new, graph=False))
+
+
+def test_counts_out_of_range(model):
+    """as the operators take them: none below 0, all of the call's rows above; what the cache is said to hold is what was written"""
+    ids = plain.tokens(2, 12).cuda()
+    cache = _cache(model, 2, 64)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device='cuda')
+    with torch.no_grad():
+        model(ids[:, :5], cache, i32(5, 5))
+        model(ids[:, 5:9], cache, i32(7, -3))
+        assert cache.held.tolist() == [9, 5]
+        got = model(torch.stack([ids[0, 9:12], ids[1, 5:8]]), cache)
+    assert plain.rel(got[0], plain.oracle(model, ids[0], 0)[9:]) < plain.BOUND and plain.rel(got[1], plain.oracle(model, ids[1, :8], 0)[5:]) < plain.BOUND
