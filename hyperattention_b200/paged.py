@@ -170,12 +170,13 @@ def paged_attn_func(q, cache, table, lengths, counts=None, softmax_scale=None):
 
     lengths  int32 [B]: tokens that each sequence holds, the new ones among them
     counts   int32 [B] or None: rows of q that are tokens of the sequence, n of each without it
+    softmax_scale  head_dim ** -0.5 without it; 0 is refused
 
     Row i < counts[b] sees positions 0 .. lengths[b] - counts[b] + i.  A row that sees none, and padding rows, have o = 0 and lse = -inf.  Consecutive
     query heads share a K/V head.  Keys are read once for 16 query rows of a K/V head, those of neighbouring tokens where a token has fewer, and again
     for the next 16: made for one to a few tokens a sequence; prompts belong to HyperAttention or flash_attn_func.  Over a cache in 4 bits,
     queries of 1e34 and more are not told from infinite ones."""
-    r = (_EXT or _ext()).attn(_handle(cache), q, table, lengths, counts, float(softmax_scale or cache.head_dim ** -0.5))
+    r = (_EXT or _ext()).attn(_handle(cache), q, table, lengths, counts, float(cache.head_dim ** -0.5 if softmax_scale is None else softmax_scale))
     if r.__class__ is int or r is NotImplemented:
         _settle(r, 'attn', cache)
         return paged_attn_func(q, cache, table, lengths, counts, softmax_scale)
