@@ -189,6 +189,9 @@ class DecoderCache:
         self.held.zero_()
 
 
+_CAPTURE_STREAMS = {}
+
+
 class _Step:
     """What the blocks of one cached forward share."""
 
@@ -339,6 +342,15 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
         out = torch.empty(b, new_tokens, dtype=torch.int64, device=input_ids.device)
         if new_tokens == 0:
             return out
+        with torch.cuda.device_of(w):                            # (whichever device is current: streams and captures are the model's)
+            self._greedy(input_ids, counts, cache, out, graph)
+            if not torch.cuda.is_current_stream_capturing():
+                check_device_status(w.device)                    # (a replay does not look at the status words)
+        return out
+
+    def _greedy(self, input_ids, counts, cache, out, graph):
+        b, new_tokens = out.shape
+        sq = input_ids.shape[1]
         logits = self(input_ids, cache, counts)
         last = logits[:, -1] if counts is None else logits[torch.arange(b, device=logits.device), counts.long().clamp(1, sq) - 1]
         ids = last.argmax(-1, keepdim=True)
@@ -353,9 +365,9 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
                 if graph and i + 2 < new_tokens:
                     torch.cuda.current_stream().synchronize()
                     replay = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(replay):
+                    # (the capture's own stream, one a device: torch's default belongs to the device of the process's first capture)
+                    if ids.device not in _CAPTURE_STREAMS:
+                        _CAPTURE_STREAMS[ids.device] = torch.cuda.Stream()
+                    with torch.cuda.graph(replay, stream=_CAPTURE_STREAMS[ids.device]):
                         ids.copy_(self._run(ids, _Step(cache, 1, None, False))[:, -1].argmax(-1, keepdim=True))
             out[:, i:i + 1] = ids
-        if not torch.cuda.is_current_stream_capturing():
-            check_device_status(w.device)                    # (a replay does not look at the status words)
-        return out
