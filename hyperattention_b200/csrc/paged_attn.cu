@@ -18,6 +18,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <numeric>
 #include <type_traits>
 
@@ -488,11 +489,39 @@ int attn_ctas(const ha_paged_params& p, int lines) {
   return (int)(most < 1 ? 1 : most < resident ? most : resident);
 }
 
+// Does the device hold a cluster of 16, which a part of a GPU need not?  Asked once a device, of the kernel with the most shared memory.
+bool clusters_of_16() {
+  static std::atomic<int> cache[64];       // 0: not asked, 1: yes, 2: no
+  int dev = 0, known = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) known = cache[dev].load(std::memory_order_relaxed);
+  if (known != 0) return known == 1;
+  auto kernel = paged_attn_kernel<__nv_bfloat16, 128, true, false>;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 16;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = 16;
+  cfg.blockDim = THREADS;
+  cfg.dynamicSmemBytes = Stage<128>::SMEM;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int held = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Stage<128>::SMEM) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&held, kernel, &cfg) != cudaSuccess) {
+    held = 0;
+    cudaGetLastError();                    // (an answer, not a failure of the call)
+  }
+  if (dev >= 0 && dev < 64) cache[dev].store(held > 0 ? 1 : 2, std::memory_order_relaxed);
+  return held > 0;
+}
+
 // CTAs that share an item as a cluster, or 0.  Short contexts and few items: a cluster joins its parts over distributed shared memory, without a workspace and a
 // second launch (1 x 515 tokens, two K/V heads: 8.2 -> 6.9 us on the device, 7.1 -> 2.7 us for the call).  Every item gets the same CTAs, however long it is, so that
 // the list of tiles, which deals them out evenly, is for what takes longer than the joining: with CLUSTER_TILES 7 a batch of 16 x 4096 goes by the list, 17.4 us for 15.3 (1 x 5000 gains:
 // 12.1 for 13.6); with 20, 1 x 8000 by clusters of 8, 19.5 us for 12.5; with 40 a batch of 32 x 8192, 37 us for 28.
-// Clusters of 16 (more than every GPU promises, but all of these) where they take no more than half of the room, since they need theirs within a part of the GPU: 1 x 515
+// Clusters of 16 (more than every GPU promises) where the device holds them and they take no more than half of the room, since they need theirs within a part of the GPU: 1 x 515
 // 7.05 -> 6.5 us, 1 x 5000 13.8 -> 10.0, 1 x 2051 in 4 bits 10.2 -> 9.2, 1 x 8000 in 4 bits 16.7 -> 12.2 (with all of the room 8 x 1000 took 13.7 us, by clusters of 8 7.7).  At
 // eight tiles a CTA the list is faster again: 1 x 8000 12.5 and 12.1 us, 1 x 16000 in 4 bits 17.2 and 15.6.
 int attn_cluster(const ha_paged_params& p) {
@@ -501,7 +530,7 @@ int attn_cluster(const ha_paged_params& p) {
   if (units > resident || tiles == 0) return 0;
   int c = 1;
   while (c < 8 && c < tiles && units * 2 * c <= resident) c *= 2;
-  if (c == 8 && tiles > 8 && units * 32 <= resident) c = 16;
+  if (c == 8 && tiles > 8 && units * 32 <= resident && clusters_of_16()) c = 16;
   return (tiles + c - 1) / c <= (c == 16 ? CLUSTER_TILES_16 : CLUSTER_TILES) ? c : 0;
 }
 
