@@ -7,6 +7,8 @@ library, libhyperattn_b200_timing.so, with the kernels' per-phase cycle counters
 ``python -m hyperattention_b200.phase_timing``); the product library never carries them.
 """
 import argparse
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -30,10 +32,21 @@ def _newer(path, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _torch_id():
+    """Where torch lies and its version, without importing it; None where there is none."""
+    spec = importlib.util.find_spec('torch')
+    return None if spec is None else f'{os.path.dirname(spec.origin)} {importlib.metadata.version("torch")} python {sys.version_info[0]}.{sys.version_info[1]}'
+
+
 def build_ext(force=False, verbose=False):
-    """The Python operators of the paged cache (paged_ext.cpp) as an extension module, next to the library whose functions it is handed."""
-    src, header = os.path.join(HERE, 'paged_ext.cpp'), os.path.join(ROOT, 'include', 'hyperattn_b200.h')
-    if not force and not _newer(EXT, [src, header]):
+    """The Python operators of the paged cache (paged_ext.cpp) as an extension module, next to the library whose functions it is handed.  Belongs to the torch that
+    it was built against (a stamp beside the object files says which) and is built anew for another; None where there is no torch: the library does without."""
+    src, header, stamp = os.path.join(HERE, 'paged_ext.cpp'), os.path.join(ROOT, 'include', 'hyperattn_b200.h'), os.path.join(HERE, 'build', '_paged_ext.stamp')
+    want = _torch_id()
+    if want is None:
+        sys.stderr.write('torch is not installed: _paged_ext.so, the Python side of the paged cache, is not built\n')
+        return None
+    if not force and not _newer(EXT, [src, header]) and os.path.exists(stamp) and open(stamp).read() == want:
         return EXT
     import sysconfig
     import torch
@@ -49,6 +62,9 @@ def build_ext(force=False, verbose=False):
         sys.stderr.write(' '.join(cmd) + '\n' + r.stdout + r.stderr)
     if r.returncode != 0:
         raise RuntimeError('g++ failed for ' + src)
+    os.makedirs(os.path.dirname(stamp), exist_ok=True)
+    with open(stamp, 'w') as f:
+        f.write(want)
     return EXT
 
 
