@@ -173,6 +173,8 @@ bool failed(const Handle& h) { return h.failed && *h.failed != 0; }
 PyObject* ext_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     want(n == 9, "append takes nine arguments");
+    const int keys = PyObject_IsTrue(a[8]);
+    if (keys < 0) return nullptr;
     Handle& h = handle_of(a[0]);
     if (failed(h)) Py_RETURN_NOTIMPLEMENTED;
     const Tensor k = rows(tensor_of(a[1], "k must be a tensor")), v = rows(tensor_of(a[2], "v must be a tensor"));
@@ -208,7 +210,6 @@ PyObject* ext_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.rope_rows = (int32_t)rope->size(0);
       p.rope_dtype = rope->scalar_type() == at::kFloat ? HA_FP32 : p.dtype;
     }
-    const bool keys = PyObject_IsTrue(a[8]) == 1;
     if (keys) {
       k_out = dense(h, k.sizes(), h.dtype);
       p.k_out = k_out.data_ptr();
