@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(32 * WARPS * ROWS) paged_combine_kernel(const 
   __syncthreads();
 #pragma unroll
   for (int x = 0; x < WARPS; ++x) m = fmaxf(m, red_m[sub][x]);
-  // pieces p = warp, warp + 4, ...: a lane D / 32 columns
+  // pieces p = warp, warp + WARPS, ...: a lane D / 32 columns
   constexpr int E = D / 32;
   float v[E], l = 0.f;
 #pragma unroll

@@ -91,16 +91,6 @@ struct Walk {
     ++line;
     settle(first, lines);
   }
-  __device__ __forceinline__ void skip(int by, const int* first, int lines, int items) {       // (the end of the list is by or more tiles away)
-    tile += by;
-    while (tile >= tiles) {
-      tile -= tiles;
-      if (++item < items) continue;
-      item = 0;
-      ++line;
-      settle(first, lines);
-    }
-  }
 };
 
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return chunk ^ (row & 7); }      // 16-byte chunk of a query row in shared memory
