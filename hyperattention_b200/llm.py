@@ -304,9 +304,9 @@ class ChatGLM2ShapedDecoder(torch.nn.Module):
         if cache is None:
             return self._run(input_ids, None)
         cache.check(self.config, b, sq)
-        prompt = cache.length == 0
-        cache.length += sq
-        return self._run(input_ids, _Step(cache, sq, counts, prompt))
+        logits = self._run(input_ids, _Step(cache, sq, counts, cache.length == 0))
+        cache.length += sq                                       # (a call that was refused on the way has added nothing)
+        return logits
 
     def _run(self, input_ids, step):
         sq = input_ids.shape[1]

@@ -47,3 +47,12 @@ def test_generate_refuses_the_cache_of_another_batch(model):
     cache = DecoderCache(model.config, 3, 16, page_size=8, device='cpu')
     with pytest.raises(AssertionError, match='another batch'):
         model.generate(torch.zeros(2, 20, dtype=torch.int64), 3, cache=cache)
+
+
+def test_a_refused_call_adds_nothing(model):
+    """the cache is as empty as before, and takes the prompt when the call is made as it should be"""
+    cache = DecoderCache(model.config, 2, 16, page_size=8, device='cpu')
+    for _ in range(3):
+        with pytest.raises(AssertionError, match='no gradient|CUDA'):
+            model(torch.zeros(2, 12, dtype=torch.int64), cache)
+        assert cache.length == 0 and not cache.held.any()
