@@ -331,8 +331,10 @@ __global__ void __launch_bounds__(THREADS, Stage<D>::CTAS)
     mbar_init(bars + 8 * 2 * NS, 4);
     mbar_fence_init();
     *abort_flag = 0;
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&km) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&vm) : "memory");
+    if (a.c.pages > 0) {                       // (a pool without pages has no maps)
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&km) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&vm) : "memory");
+    }
   }
   // The kernel behind is let in at the end: its CTAs would take the places that come free one by one, several on some SMs and none on others
   // (1 x 131072 tokens, 32 heads x 64, passes back to back: 242 us with an early release, 165 without).
