@@ -205,6 +205,7 @@ PyObject* ext_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       want(rope->dim() == 3 && rope->size(2) == 2 && rope->is_contiguous() && rope->device() == h.device, "rope must be contiguous [positions, rot / 2, 2]");
       want((rope->scalar_type() == at::kFloat || rope->scalar_type() == h.dtype) && 2 * rope->size(1) <= p.d && rope->size(0) <= INT32_MAX,
            "rope must be fp32 or of the cache's type, for at most head_dim elements");
+      want(rope->size(0) > 0 || rope->size(1) == 0 || B * m == 0, "rope must have the tokens' positions");     // (an empty tensor has no address, which would mean no rotation)
       p.rope = rope->data_ptr();
       p.rot = (int32_t)(2 * rope->size(1));
       p.rope_rows = (int32_t)rope->size(0);

@@ -36,3 +36,15 @@ def test_a_pool_without_pages(bits, columns):
         call()
         with pytest.raises(RuntimeError, match='outside'):
             ha.check_device_status()
+
+
+def test_a_rotation_without_positions():
+    """refused, not taken for no rotation; without elements to rotate, or without tokens, there is nothing to look up"""
+    cache = ha.PagedCache.allocate(2, 16, 2, 64)
+    x = torch.ones(1, 1, 2, 64, dtype=torch.bfloat16, device='cuda')
+    table, length = torch.zeros(1, 2, dtype=torch.int32, device='cuda'), torch.zeros(1, dtype=torch.int32, device='cuda')
+    rope = torch.empty(8, 32, 2, device='cuda')
+    with pytest.raises(AssertionError, match='rope'):
+        ha.paged_append(cache, x, x, table, length, rope=rope[:0], q=x)
+    assert torch.equal(ha.paged_append(cache, x, x, table, length, rope=rope[:, :0].contiguous(), q=x), x)
+    assert ha.paged_append(cache, x[:, :0], x[:, :0], table, length, rope=rope[:0], q=x[:, :0]).shape == (1, 0, 2, 64)
