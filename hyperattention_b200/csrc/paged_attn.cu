@@ -13,8 +13,8 @@
 // Here: 16-bit rows, the joining of parts, the entry points.  (4-bit rows: paged_attn4.cu.)  A CTA: four warps that compute, each a quarter of a tile's
 // keys with its own running maximum and sums, which are joined at the item's end; and one that fetches tiles into a ring of NS stages, across
 // items, by tensor copies (128-byte swizzle; boxes of as many rows as both a page and a tile are made of, so that any page size will do).
-// 1 x 131072 tokens, 32 heads x 64: 167 us, 6.4 TB/s (98 % of a copy's rate).  Batch of 32 x up to 8192, two K/V heads x 128: 27.6 us, 3.5 TB/s: what remains is the
-// latency of a kernel's start, of a part's end and of the joining.
+// 1 x 131072 tokens, 32 heads x 64: 166 to 172 us from machine to machine, 6.2 to 6.5 TB/s (95 to 99 % of a copy's rate).  Batch of 32 x up to 8192, two
+// K/V heads x 128: 27.2 us, 3.5 TB/s: what remains is the latency of a kernel's start, of a part's end and of the joining.
 #include <string.h>
 
 #include <algorithm>

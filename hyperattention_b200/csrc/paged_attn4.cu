@@ -13,8 +13,8 @@
 // begin and its end the warps do not wait for one another.  cp.async, whose copies of a warp's 32 or 64 neighbouring rows need two addresses: bulk copies,
 // of which a warp's part of a tile takes four, cost some 100 instructions where these cost 40.
 //
-// Bound by instructions: batch of 64 x up to 32768, two K/V heads x 128, 16 query heads each: 80 us, 2.6 TB/s; without the copies 84, the copies alone 50.  1 x 262144, 32 heads
-// x 64: 137 us, 4.4 TB/s; 124 and 97.  (Queries as the sixteen rows of the products and tiles fetched by
+// Bound by instructions: batch of 64 x up to 32768, two K/V heads x 128, 16 query heads each: 81 us, 2.6 TB/s; without the copies 84, the copies alone 50.  1 x 262144, 32 heads
+// x 64: 136 to 148 us from machine to machine, 4.1 to 4.4 TB/s; 124 and 97 on the first of them.  (Queries as the sixteen rows of the products and tiles fetched by
 // a fifth warp took 105 and 323 us.)
 #include <type_traits>
 

@@ -150,10 +150,11 @@ __device__ __forceinline__ uint2 quantise(const float (&x)[PART], __half2& scale
 }
 
 // One block a token, D / 16 lanes a row, sixteen elements a lane, which keeps its cosines and sines for all the heads that it meets; two rows of a
-// lane under way at once.  Bound by the bytes of q, k and v for prompts, by the chain length -> page -> store for single tokens.  32768 tokens, 32 + 2 + 2
-// heads x 128: 98 us, 6.3 TB/s; 2 x 8191 tokens, 32 + 32 + 32 heads x 64, into 4 bits: 77 us, 3.7 TB/s, the codes' arithmetic beside the copies; one token of 32
-// sequences: 2.4 us.  (16 bits: 20 warps an SM, 102 registers: 24 x 2319 tokens, 12 + 2 + 2 heads x 128, 82.8 -> 75.3 us; 24 warps spill.  4 bits: 16
-// warps, 128 registers: by 18 or 20 with spilled ones 107 -> 114 us, by fewer with more 124.)
+// lane under way at once.  Bound by the bytes of q, k and v for long prompts, by the chain length -> page -> store for single tokens.  32768 tokens, 32 + 2 + 2
+// heads x 128: 97 to 103 us from machine to machine, 5.9 to 6.3 TB/s; 2 x 8191 tokens, 32 + 32 + 32 heads x 64, into 4 bits: 77 to 80 us, 3.8 to 4.0 TB/s: a block's
+// rounds of loads one after another, with the codes' arithmetic between them; one token of 32 sequences: 2.4 us.  (16 bits: 20 warps an SM, 96 registers:
+// 24 x 2319 tokens, 12 + 2 + 2 heads x 128, 82.8 -> 75.3 us; 24 warps spill.  4 bits: 16 warps, 120 of their 128 registers: by 18 or 20 with spilled ones
+// 107 -> 114 us, by fewer with more 124.)
 template <typename T, int D, int BITS, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS, (BITS == 16 ? 640 : 512) / THREADS) paged_append_kernel(const AppendArgs a) {
   chain_begin();
@@ -295,7 +296,7 @@ __device__ __forceinline__ uint4 values8(uint32_t w, float2 f) {
 }
 
 // D / 16 lanes a row, eight elements of each half of it a lane; ROWS rows of K and V a thread, whose loads are under way together.  Bound by the bytes written: 2 x 8322
-// rows, 32 heads x 64, from 4 bits: 31 us, 5.6 TB/s.
+// rows, 32 heads x 64, from 4 bits: 30 to 31 us, 5.6 to 5.9 TB/s.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
   chain_begin();
